@@ -270,6 +270,121 @@ int mvllm_hip_linear_dev(int fmt, const void *w, const void *scales, int O, int 
 int mvllm_hip_rmsnorm_dev(const float *x, const float *w, float *y, int rows, int n, float eps,
                           void *stream);
 
+/* ---- attention over keys and values held in 4 bits (device, enqueued on `stream`; 1 =
+ *      enqueued, 0 = bad arguments, see mvllm_hip_last_error) -------------------------------
+ * What a decoder layer runs in front of its routed experts, for engines that keep the layer
+ * on the GPU: norm and rotate the query and key heads, put keys and values into a paged cache
+ * in the library's own 4-bit formats, attend over it, and drop its least attended tokens.
+ * No counterpart in the reference (its caches are host memory).
+ *
+ * The calls keep no state and share no scratch: calls that touch the same buffers are ordered
+ * by the caller, any others may overlap, on any streams and threads.  Nothing is read on the
+ * host and nothing allocated, so all of them can be captured into graphs; lengths and tables
+ * are device memory and may change between replays.  Launches go to the device of
+ * mvllm_hip_init whatever the current device is; a stream of another device is refused.
+ *
+ * dtype: 0 f32, 1 bf16 (rows of heads; weights, scores and sums are f32).  Rows of heads are
+ * [heads][head_dim], 16-byte aligned, token t's at t * stride elements (stride a multiple of
+ * 16 bytes, so they may be columns of a wider projection); head_dim is 64, 128, 192 or 256. */
+
+/* The cache: n_pages pages of `page` tokens (a multiple of 16, at most 1024) in caller-owned
+ * device memory, 16-byte aligned:
+ *   k, v    codes [n_pages][n_kv][page][head_dim / 2], low nibble = even element
+ *   ks, vs  scales [n_pages][n_kv][page][head_dim / 64] f32 (fmt 4, value (n - 8) * scale) or
+ *           [head_dim / 32] ue8m0 bytes (fmt 7)
+ *   score   [n_pages][n_kv][page] f32, the tokens' accumulated attention weights, or NULL
+ * mvllm_kv4_geom gives the sizes of a page.
+ *
+ * A call's sequences: sequence b has lens[b] tokens, token t in slot t % page of page
+ * table[b * max_pages + t / page]; its new tokens are the call's rows [q_start[b],
+ * q_start[b + 1]) (q_start does not fall and ends at most at n_tok) and the LAST of its
+ * lens[b].  Rows ahead of q_start[0] or behind q_start[n_seq] belong to no sequence and are
+ * left as they are.  A table entry outside [0, n_pages), or a token past the table, is a token
+ * that is not there: not written, not seen, read as zeros.  A row whose token would be before
+ * its sequence's first (more rows than lens[b]) has no place in the cache. */
+typedef struct mvllm_kv4 {
+    void *k, *ks, *v, *vs;
+    float *score;
+    int fmt, n_kv, head_dim, page, n_pages;
+} mvllm_kv4;
+
+/* Bytes of one page of {k, ks, v, vs} (bytes may be NULL); returns their sum, or -1 for a bad
+ * shape.  Host only. */
+long long mvllm_kv4_geom(int fmt, int n_kv, int head_dim, int page, long long bytes[4]);
+
+/* Every head x of n_tok tokens' n_q query and n_kv key heads: y = x / sqrt(mean(x^2) + eps) *
+ * w (wq / wk [head_dim], NULL: none), then, unless freq is NULL, the rotation of its first
+ * `rot` elements (a multiple of 16): pair j turns by the angle pos[t] * freq[j] (freq
+ * [rot / 2], usually base^(-2 j / rot); the angle is formed in 64 bits), (a, b) -> (a cos - b
+ * sin, b cos + a sin), where (a, b) are elements (j, j + rot / 2), or (2 j, 2 j + 1) with
+ * `interleaved`.  One pass; sums and the rotation in f32, rounded once to dtype.  qo / ko may be
+ * q / k themselves (with their strides); otherwise outputs overlap no input.  n_q or n_kv may
+ * be 0 (its pointers are then not used). */
+int mvllm_hip_qk_norm_rope_dev(int dtype, int n_tok, int head_dim, const void *q,
+                               long long q_stride, int n_q, void *qo, long long qo_stride,
+                               const void *k, long long k_stride, int n_kv, void *ko,
+                               long long ko_stride, const float *wq, const float *wk, float eps,
+                               const int *pos, const double *freq, int rot, int interleaved,
+                               void *stream);
+
+/* The new tokens' keys and values (n_kv heads a row) into their places, quantized along
+ * head_dim: fmt 4, groups of 64: scale = (largest magnitude) / 7 in f32, n = x / scale rounded
+ * to nearest (ties to even, decided exactly) + 8; fmt 7, groups of 32: the activation
+ * quantizer's rule (mvllm_hip_quantize_mxfp4).  NaN is held as 0, magnitudes above 6 * 2^125
+ * (infinities too) as that; an int4 group of nothing above 2^-100 as zeros.  Clears the tokens'
+ * scores where the cache has them. */
+int mvllm_hip_kv4_append_dev(const mvllm_kv4 *cache, int dtype, const void *k, long long k_stride,
+                             const void *v, long long v_stride, int n_tok, const int *q_start,
+                             const int *lens, const int *table, int n_seq, int max_pages,
+                             void *stream);
+
+/* The rows' keys and values as the cache holds them, into k / v [n_tok][n_kv][head_dim] (to
+ * move a sequence to another cache, or to look at it; with q_start the running sum of lens,
+ * whole sequences).  f32 is exact. */
+int mvllm_hip_kv4_read_dev(const mvllm_kv4 *cache, int dtype, void *k, void *v, int n_tok,
+                           const int *q_start, const int *lens, const int *table, int n_seq,
+                           int max_pages, void *stream);
+
+/* Attention of the new tokens (already appended) over the cache: out [n_tok][n_q][head_dim],
+ * query head h of the new token at position p (its index among the sequence's lens[b] tokens)
+ * = sum_j P_j v_j over the tokens j <= p (and j > p - window where window > 0) of kv head h /
+ * (n_q / n_kv), P = softmax(scale * q . k_j).  A row that sees no token gives zeros.
+ * Products: the codes enter the bf16 matrix cores exactly; f32 queries and probabilities as
+ * three bf16 terms (all 24 bits), bf16 queries exactly and their probabilities as two terms;
+ * sums, maxima and exponentials are f32.
+ * weights: 1 adds to score, 2 stores into it, for each of the sequences' tokens, the sum of its
+ * P over the call's new tokens and the kv head's group of query heads (0 where none sees it).
+ * Sequences that share pages may attend together with weights 0; their scores would be two
+ * writers of one place.
+ * max_new / max_len: the most new tokens and tokens of a sequence that the launch is sized
+ * for; larger ones run too, with less of the chip.  work: device memory of
+ * mvllm_hip_kv4_attention_work bytes for the same sizes, the call's own until it ends (two
+ * graphs that may run at once need two). */
+int mvllm_hip_kv4_attention_dev(const mvllm_kv4 *cache, int dtype, const void *q,
+                                long long q_stride, int n_q, int n_tok, const int *q_start,
+                                const int *lens, const int *table, int n_seq, int max_pages,
+                                int max_new, int max_len, float scale, int window, int weights,
+                                void *out, void *work, size_t work_bytes, void *stream);
+/* Bytes of that workspace (0: none needed), or -1 for sizes the call refuses.  Host only. */
+long long mvllm_hip_kv4_attention_work(int n_kv, int head_dim, int n_q, int n_tok, int n_seq,
+                                       int max_new, int max_len, int weights);
+
+/* Eviction by accumulated weight.  Of each sequence of more than `keep` tokens every kv head
+ * keeps its last `recent` (<= keep) tokens and, of the others, the keep - recent of largest
+ * score (ties: the lowest index; NaN is least; a token that is not there likewise).  The kept
+ * tokens' codes, scales and scores move, in order, to tokens 0.. of the pages that
+ * dst_table [n_seq][dst_max_pages] names: pages of the same cache that no sequence of the call
+ * is read from.  A shorter sequence moves whole.  kept [n_seq][n_kv][keep] = the tokens kept,
+ * ascending, then -1; new_lens[b] = min(lens[b], keep) (not lens itself: heads still read
+ * it).  The source pages are left as they are; a moved token that is not there leaves its
+ * place as it is.  Positions: a cached key keeps its rotation; the engine goes on counting
+ * positions for new tokens, while lens, causality and windows count the tokens held.
+ * max_len: the most tokens the launch is sized for; longer sequences run too, slower. */
+int mvllm_hip_kv4_evict_dev(const mvllm_kv4 *cache, const int *lens, const int *table, int n_seq,
+                            int max_pages, int max_len, int keep, int recent,
+                            const int *dst_table, int dst_max_pages, int *kept, int *new_lens,
+                            void *stream);
+
 /* Expert blob geometry (byte offsets of the six pieces inside one expert blob):
  * fmt 4 = GLM gate_p|gate_s|up_p|up_s|down_p|down_s (src/model/glm53.cpp:56-78,
  * 116-132); fmt 7 = K3 w1p|w1s|w2p|w2s|w3p|w3s with gate=w1, down=w2, up=w3

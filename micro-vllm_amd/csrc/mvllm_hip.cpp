@@ -26,6 +26,7 @@
 
 namespace mvllm_hip {
 void set_error(const std::string &s);
+int ready_device();
 }
 
 using namespace mvllm_hip;
@@ -291,6 +292,13 @@ Ctx &ctx() {
     static Ctx c;
     return c;
 }
+
+}  // namespace
+
+// the device of mvllm_hip_init, or -1 before it
+int mvllm_hip::ready_device() { return ctx().ready ? ctx().device : -1; }
+
+namespace {
 
 // ---- device memory of the no-allocation entry (mvllm_hip_moe_block_dev_noalloc) -----
 // One array per device, held until the process ends: the plan's device copy in the first

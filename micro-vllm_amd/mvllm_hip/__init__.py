@@ -25,6 +25,8 @@ LIB_PATH = os.path.join(PKG_DIR, "libmvllm_hip.so")
 HEADER = os.path.join(os.path.dirname(PKG_DIR), "include", "mvllm_hip.h")
 
 ACT_SILU, ACT_CLAMP_SWIGLU, ACT_SITU = 0, 1, 2
+F32, BF16 = 0, 1
+WEIGHTS_NONE, WEIGHTS_ADD, WEIGHTS_STORE = 0, 1, 2
 STAT_NAMES = ["calls", "rows", "h2d_weight_bytes", "h2d_act_bytes", "d2h_bytes", "promotions",
               "resident_hits", "misses", "evictions", "ms_gate_up", "ms_down", "ms_combine",
               "ms_prep", "launches_gate_up", "launches_down", "host_ms", "host_wait_ms",
@@ -79,6 +81,15 @@ _SIGS = {
     "mvllm_hip_host_reuse": (_i, [_p, _sz]),
     "mvllm_hip_tier_table": (_i, [_i, _i, _p, _p, _p]),
     "mvllm_hip_tier_table_done": (_i, [_i, _p]),
+    "mvllm_kv4_geom": (_ll, [_i, _i, _i, _i, _p]),
+    "mvllm_hip_qk_norm_rope_dev": (_i, [_i, _i, _i, _p, _ll, _i, _p, _ll, _p, _ll, _i, _p, _ll, _p,
+                                        _p, _f, _p, _p, _i, _i, _p]),
+    "mvllm_hip_kv4_append_dev": (_i, [_p, _i, _p, _ll, _p, _ll, _i, _p, _p, _p, _i, _i, _p]),
+    "mvllm_hip_kv4_read_dev": (_i, [_p, _i, _p, _p, _i, _p, _p, _p, _i, _i, _p]),
+    "mvllm_hip_kv4_attention_dev": (_i, [_p, _i, _p, _ll, _i, _i, _p, _p, _p, _i, _i, _i, _i, _f,
+                                         _i, _i, _p, _p, _sz, _p]),
+    "mvllm_hip_kv4_attention_work": (_ll, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "mvllm_hip_kv4_evict_dev": (_i, [_p, _p, _p, _i, _i, _i, _i, _i, _p, _i, _p, _p, _p]),
     "mvllm_hip_moe_block_routed_dev": (_i, [_i, _i, _i, _p, _i, _p, _p, _p, _p, _i, _p, _p, _i,
                                             _p, _p, _i, _i, _f, _f, _p, _p]),
 }
@@ -305,6 +316,87 @@ def linear_dev(fmt, w, scales, O, K, x, n, y, stream=None):
 def rmsnorm_dev(x, w, y, rows, n, eps, stream=None):
     _check(lib().mvllm_hip_rmsnorm_dev(_ptr(x), _ptr(w), _ptr(y), rows, n, eps,
                                        _stream(stream)), "mvllm_hip_rmsnorm_dev")
+
+
+class _KV4(C.Structure):
+    _fields_ = [("k", _p), ("ks", _p), ("v", _p), ("vs", _p), ("score", _p), ("fmt", _i),
+                ("n_kv", _i), ("head_dim", _i), ("page", _i), ("n_pages", _i)]
+
+
+class KV4:
+    """A paged 4-bit key/value cache (mvllm_kv4): keeps its arrays (torch tensors, or
+    addresses with n_pages given) and the structure the calls take."""
+
+    def __init__(self, fmt, n_kv, head_dim, page, k, ks, v, vs, score=None, n_pages=None):
+        self.arrays = (k, ks, v, vs, score)
+        self.fmt, self.n_kv, self.head_dim, self.page = fmt, n_kv, head_dim, page
+        self.n_pages = len(k) if n_pages is None else n_pages
+        self.desc = _KV4(_ptr(k), _ptr(ks), _ptr(v), _ptr(vs), _ptr(score), fmt, n_kv, head_dim,
+                         page, self.n_pages)
+        self.ref = C.addressof(self.desc)
+
+
+def kv4_geom(fmt, n_kv, head_dim, page):
+    """-> (bytes of a page, [k, ks, v, vs] bytes of it); -1 for a bad shape."""
+    b = np.zeros(4, np.int64)
+    n = lib().mvllm_kv4_geom(fmt, n_kv, head_dim, page, _ptr(b))
+    return int(n), b
+
+
+def qk_norm_rope_dev(dtype, n_tok, head_dim, q, q_stride, n_q, qo, qo_stride, k, k_stride, n_kv,
+                     ko, ko_stride, wq, wk, eps, pos, freq, rot, interleaved=False, stream=None):
+    """RMSNorm of every query and key head and the rotation (see mvllm_hip_qk_norm_rope_dev);
+    strides in elements between tokens.  Enqueued."""
+    _check(lib().mvllm_hip_qk_norm_rope_dev(dtype, n_tok, head_dim, _ptr(q), q_stride, n_q,
+                                            _ptr(qo), qo_stride, _ptr(k), k_stride, n_kv, _ptr(ko),
+                                            ko_stride, _ptr(wq), _ptr(wk), eps, _ptr(pos),
+                                            _ptr(freq), rot, int(interleaved), _stream(stream)),
+           "mvllm_hip_qk_norm_rope_dev")
+
+
+def kv4_append_dev(cache, dtype, k, k_stride, v, v_stride, n_tok, q_start, lens, table, n_seq,
+                   max_pages, stream=None):
+    """New keys and values into the cache (see mvllm_hip_kv4_append_dev); enqueued."""
+    _check(lib().mvllm_hip_kv4_append_dev(cache.ref, dtype, _ptr(k), k_stride, _ptr(v), v_stride,
+                                          n_tok, _ptr(q_start), _ptr(lens), _ptr(table), n_seq,
+                                          max_pages, _stream(stream)), "mvllm_hip_kv4_append_dev")
+
+
+def kv4_read_dev(cache, dtype, k, v, n_tok, q_start, lens, table, n_seq, max_pages, stream=None):
+    """The rows' keys and values as the cache holds them (see mvllm_hip_kv4_read_dev)."""
+    _check(lib().mvllm_hip_kv4_read_dev(cache.ref, dtype, _ptr(k), _ptr(v), n_tok, _ptr(q_start),
+                                        _ptr(lens), _ptr(table), n_seq, max_pages,
+                                        _stream(stream)), "mvllm_hip_kv4_read_dev")
+
+
+def kv4_attention_work(n_kv, head_dim, n_q, n_tok, n_seq, max_new, max_len, weights=False):
+    """Bytes of the workspace of kv4_attention_dev for these sizes."""
+    n = lib().mvllm_hip_kv4_attention_work(n_kv, head_dim, n_q, n_tok, n_seq, max_new, max_len,
+                                           int(weights))
+    if n < 0:
+        raise HipError("mvllm_hip_kv4_attention_work: bad sizes")
+    return n
+
+
+def kv4_attention_dev(cache, dtype, q, q_stride, n_q, n_tok, q_start, lens, table, n_seq,
+                      max_pages, max_new, max_len, scale, window, weights, out, work, work_bytes,
+                      stream=None):
+    """Causal attention of the new tokens over the cache (see mvllm_hip_kv4_attention_dev)."""
+    _check(lib().mvllm_hip_kv4_attention_dev(cache.ref, dtype, _ptr(q), q_stride, n_q, n_tok,
+                                             _ptr(q_start), _ptr(lens), _ptr(table), n_seq,
+                                             max_pages, max_new, max_len, scale, window, weights,
+                                             _ptr(out), _ptr(work), work_bytes, _stream(stream)),
+           "mvllm_hip_kv4_attention_dev")
+
+
+def kv4_evict_dev(cache, lens, table, n_seq, max_pages, max_len, keep, recent, dst_table,
+                  dst_max_pages, kept, new_lens, stream=None):
+    """Each head's most attended and most recent tokens to fresh pages (see
+    mvllm_hip_kv4_evict_dev); enqueued."""
+    _check(lib().mvllm_hip_kv4_evict_dev(cache.ref, _ptr(lens), _ptr(table), n_seq, max_pages,
+                                         max_len, keep, recent, _ptr(dst_table), dst_max_pages,
+                                         _ptr(kept), _ptr(new_lens), _stream(stream)),
+           "mvllm_hip_kv4_evict_dev")
 
 
 def bf16_planes(fmt, terms, x_dev, n, K, planes_dev):
