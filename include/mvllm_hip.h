@@ -328,8 +328,8 @@ int mvllm_hip_qk_norm_rope_dev(int dtype, int n_tok, int head_dim, const void *q
                                void *stream);
 
 /* The new tokens' keys and values (n_kv heads a row) into their places, quantized along
- * head_dim: fmt 4, groups of 64: scale = (largest magnitude) / 7 in f32, n = x / scale rounded
- * to nearest (ties to even, decided exactly) + 8; fmt 7, groups of 32: the activation
+ * head_dim: fmt 4, groups of 64: scale = (largest magnitude) * (1 / 7), both f32, n = x / scale
+ * rounded to nearest (ties to even, decided exactly) + 8; fmt 7, groups of 32: the activation
  * quantizer's rule (mvllm_hip_quantize_mxfp4).  NaN is held as 0, magnitudes above 6 * 2^125
  * (infinities too) as that; an int4 group of nothing above 2^-100 as zeros.  Clears the tokens'
  * scores where the cache has them. */

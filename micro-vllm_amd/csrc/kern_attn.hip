@@ -13,8 +13,6 @@ namespace mvllm_hip {
 
 namespace {
 
-typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-
 __device__ __forceinline__ f4v mfma(bf16x8 a, bf16x8 b, f4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -86,7 +84,7 @@ __device__ __forceinline__ void span_of(const AttnArgs &A, const Tile &t, int r0
 }
 
 // B operands of 16 rows of queries: lane (column c, group of lanes kg) holds, of each 64
-// elements g, the 16 from 64 g + 16 kg, as two operands (int4: in decode_b4_signed's order).
+// elements g, the 16 from 64 g + 16 kg, as two operands (int4: in decode_b<4>'s order).
 template <int FMT, int NG, int TQ, typename T>
 __device__ __forceinline__ void load_q(const AttnArgs &A, const Tile &t, int row, bool live,
                                        bf16x8 (&q)[NG][2][TQ]) {
@@ -138,19 +136,37 @@ template <int FMT, int NG> struct Keys {
     }
 };
 
+// -8 times each row's sum of queries in each group of 64: what the sums of products with int4
+// codes n start from, so that they end as those with n - 8 (one instruction for 4 codes in place
+// of five).
+template <int NG, int TQ>
+__device__ __forceinline__ void offsets_of(const bf16x8 (&q)[NG][2][TQ], float (&k8)[NG]) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        float sum = 0.f;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int k = TQ - 1; k >= 0; --k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    sum += (float)q[g][s][k][e];
+        k8[g] = -8.f * col_sum(sum);
+    }
+}
+
 // Products of 16 tokens' keys with 16 rows of queries: S[i] is token 4 kg + i, row c.  An int4
 // group's codes are summed exactly and its scale applied to the sum; an MXFP4 code times its
 // scale is exact in bf16.
 template <int FMT, int NG, int TQ>
-__device__ __forceinline__ f4v dot_keys(const Keys<FMT, NG> &k, const bf16x8 (&q)[NG][2][TQ]) {
+__device__ __forceinline__ f4v dot_keys(const Keys<FMT, NG> &k, const bf16x8 (&q)[NG][2][TQ],
+                                        const float (&k8)[NG]) {
     f4v sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-        const bf16x8 a0 = FMT == 4 ? decode_b4_signed(k.w[g].x) : decode_b<7>(k.w[g].x, k.s[g]);
-        const bf16x8 a1 = FMT == 4 ? decode_b4_signed(k.w[g].y) : decode_b<7>(k.w[g].y, k.s[g]);
-        f4v acc = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (FMT == 7)
-            acc = sum;
+        const bf16x8 a0 = decode_b<FMT>(k.w[g].x, FMT == 7 ? k.s[g] : 0.f);
+        const bf16x8 a1 = decode_b<FMT>(k.w[g].y, FMT == 7 ? k.s[g] : 0.f);
+        f4v acc = FMT == 4 ? f4v{k8[g], k8[g], k8[g], k8[g]} : sum;
 #pragma unroll
         for (int t = TQ - 1; t >= 0; --t) {
             acc = mfma(a0, q[g][0][t], acc);
@@ -168,11 +184,17 @@ __device__ __forceinline__ f4v dot_keys(const Keys<FMT, NG> &k, const bf16x8 (&q
 }
 
 // 32 tokens' values as the lanes need them: lane (m, kg), of tokens 4 kg + i and 16 + 4 kg + i
-// (the tokens whose probabilities the lane holds), elements 64 g + 4 m + j.
-template <int FMT, int NG> struct Vals {
+// (the tokens whose probabilities the lane holds), and what is summed of them.
+//
+// int4: elements 64 g + 4 m + j, so that a product's rows share one group and the group's scale
+// can go to the probabilities.  UNS: the codes enter as n, without the offset of 8, and one
+// more product of the probabilities with a constant takes 8 of their sum off again; the sums
+// are then off by 2^-24 of sum p s n in place of sum p s |n - 8|, too much for f32 outputs.
+template <int FMT, int NG, bool UNS> struct Vals;
+
+template <int NG, bool UNS> struct Vals<4, NG, UNS> {
     uint16_t w[NG][8];
-    float s[FMT == 4 ? 8 * NG : 1];      // int4: [token][group]
-    uint2 b[FMT == 4 ? 1 : 2][NG];       // MXFP4: bytes [token][2 NG] of 4 tokens
+    float s[8 * NG];  // [token][group]
 
     __device__ __forceinline__ void load(const Kv4View &c, size_t row, int half) {
         const int lane = threadIdx.x & 63, m = lane & 15, kg = lane >> 4;
@@ -184,76 +206,257 @@ template <int FMT, int NG> struct Vals {
             for (int i = 0; i < 4; ++i)
                 w[g][4 * half + i] =
                     *reinterpret_cast<const uint16_t *>(p + i * (32 * NG) + 32 * g);
-        if constexpr (FMT == 4) {
-            const float4 *sp = reinterpret_cast<const float4 *>(c.vs + row * (4 * NG));
+        const float4 *sp = reinterpret_cast<const float4 *>(c.vs + row * (4 * NG));
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const float4 v = sp[g];
+            const int o = 4 * NG * half + 4 * g;
+            s[o] = v.x; s[o + 1] = v.y; s[o + 2] = v.z; s[o + 3] = v.w;
+        }
+    }
+    __device__ __forceinline__ void bound() {}  // add() leaves a masked token's scale out
+
+    struct Acc {
+        f4v o[NG][4], e[NG];
+
+        __device__ __forceinline__ void clear() {
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const float4 v = sp[g];
-                const int o = 4 * NG * half + 4 * g;
-                s[o] = v.x; s[o + 1] = v.y; s[o + 2] = v.z; s[o + 3] = v.w;
+                e[g] = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    o[g][j] = f4v{0.f, 0.f, 0.f, 0.f};
             }
-        } else {
-            const uint2 *sp = reinterpret_cast<const uint2 *>(c.vs + row * (2 * NG));
+        }
+        __device__ __forceinline__ void scale(float f) {
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                e[g] *= f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    o[g][j] *= f;
+            }
+        }
+        template <int TP>
+        __device__ __forceinline__ void add(const Vals &v, const float (&p)[8], bool whole) {
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                float ps[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    ps[i] = p[i] * v.s[i * NG + g];
+                __builtin_amdgcn_sched_barrier(0);  // one group's operands at a time
+                if (!whole) {  // a masked token's scale may be anything
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        ps[i] = p[i] == 0.f ? 0.f : ps[i];
+                }
+                bf16x8 b[TP], a[4];
+                split8<TP>(ps, b);
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {  // tokens 2 h and 2 h + 1
+                    const uint32_t x = (uint32_t)v.w[g][2 * h] | ((uint32_t)v.w[g][2 * h + 1] << 16);
+                    const uint32_t y = __builtin_amdgcn_perm(x, x, 0x03010200u);  // pairs of bytes
+                    const int lo = (int)(UNS ? y & 0x0f0f0f0fu : int4_signed_codes(y));
+                    const int hi = (int)(UNS ? (y >> 4) & 0x0f0f0f0fu : int4_signed_codes(y >> 4));
+                    const bf16x2 c[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, false),
+                                         __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, false),
+                                         __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, true),
+                                         __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, true)};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        a[j][2 * h] = c[j][0];
+                        a[j][2 * h + 1] = c[j][1];
+                    }
+                }
+                bf16x8 minus8;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    minus8[i] = (__bf16)-8.f;
+#pragma unroll
+                for (int k = TP - 1; k >= 0; --k) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        o[g][j] = mfma(a[j], b[k], o[g][j]);
+                    if constexpr (UNS)
+                        e[g] = mfma(minus8, b[k], e[g]);
+                }
+            }
+        }
+        // f(d, four sums from element d on) over the lane's elements
+        template <typename F> __device__ __forceinline__ void pieces(int kg, F &&f) const {
 #pragma unroll
             for (int g = 0; g < NG; ++g)
-                b[half][g] = sp[g];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float4 y = make_float4(o[g][0][i], o[g][1][i], o[g][2][i], o[g][3][i]);
+                    if constexpr (UNS) {
+                        y.x += e[g][i]; y.y += e[g][i]; y.z += e[g][i]; y.w += e[g][i];
+                    }
+                    f(64 * g + 16 * kg + 4 * i, y);
+                }
         }
-    }
-    // MXFP4 scale of token t (0..7) for the lane's elements of group g.  Bytes above 252,
-    // which no append writes, count as 252: a masked token's value stays finite.
-    __device__ __forceinline__ float scale7(int t, int g) const {
-        const int m = threadIdx.x & 15, h = (t & 3) * NG + g;  // 16-bit piece of the 4 tokens
-        const uint2 v = b[t >> 2][h / 4];
-        const uint32_t d = (h & 2) ? v.y : v.x;
-        const uint32_t e = (d >> (16 * (h & 1) + 8 * (m >> 3))) & 0xffu;
-        return __uint_as_float(min(e, 252u) << 23);
-    }
+    };
 };
 
-// A operands of one group's values: a[j] holds element 64 g + 4 m + j of the 8 tokens.
-template <int FMT, int NG>
-__device__ __forceinline__ void decode_vals(const Vals<FMT, NG> &v, int g, bf16x8 (&a)[4]) {
+// MXFP4: elements 128 c + 8 m + j, and of a last 64 (head_dim 64 or 192) 4 m + j; a code times
+// its scale is exact in bf16, so the scale goes to the code.
+template <int NG, bool UNS> struct Vals<7, NG, UNS> {
+    static constexpr int NC = NG / 2, ODD = NG & 1;
+    uint32_t w[NC + ODD][8];
+    uint32_t b[2][2 * NG];  // scale bytes [token][2 NG] of 4 tokens
+    uint32_t most;          // largest scale byte that counts
+
+    __device__ __forceinline__ void load(const Kv4View &c, size_t row, int half) {
+        const int lane = threadIdx.x & 63, m = lane & 15, kg = lane >> 4;
+        row += 4 * kg;
+        const uint8_t *p = c.v + row * (32 * NG);
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {  // tokens 2 p and 2 p + 1
-        const uint32_t x = (uint32_t)v.w[g][2 * p] | ((uint32_t)v.w[g][2 * p + 1] << 16);
-        uint32_t o[4];
-        if constexpr (FMT == 4) {
-            const uint32_t y = __builtin_amdgcn_perm(x, x, 0x03010200u);  // byte pairs of a place
-            const int lo = (int)int4_signed_codes(y), hi = (int)int4_signed_codes(y >> 4);
-            o[0] = as_u32(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, false));
-            o[1] = as_u32(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, false));
-            o[2] = as_u32(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, true));
-            o[3] = as_u32(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, true));
-        } else {
-            const float s0 = v.scale7(2 * p, g), s1 = v.scale7(2 * p + 1, g);
-            const uint32_t c0 = as_u32(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, s0, 0));
-            const uint32_t c1 = as_u32(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, s0, 1));
-            const uint32_t d0 = as_u32(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, s1, 2));
-            const uint32_t d1 = as_u32(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, s1, 3));
-            o[0] = __builtin_amdgcn_perm(d0, c0, 0x05040100u);
-            o[1] = __builtin_amdgcn_perm(d0, c0, 0x07060302u);
-            o[2] = __builtin_amdgcn_perm(d1, c1, 0x05040100u);
-            o[3] = __builtin_amdgcn_perm(d1, c1, 0x07060302u);
-        }
+        for (int i = 0; i < 4; ++i) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const bf16x2 b = as_bf2(o[j]);
-            a[j][2 * p] = b[0];
-            a[j][2 * p + 1] = b[1];
+            for (int n = 0; n < NC; ++n)
+                w[n][4 * half + i] =
+                    *reinterpret_cast<const uint32_t *>(p + i * (32 * NG) + 64 * n + 4 * m);
+            if constexpr (ODD)
+                w[NC][4 * half + i] =
+                    *reinterpret_cast<const uint16_t *>(p + i * (32 * NG) + 64 * NC + 2 * m);
         }
+        const uint2 *sp = reinterpret_cast<const uint2 *>(c.vs + row * (2 * NG));
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const uint2 v = sp[g];
+            b[half][2 * g] = v.x;
+            b[half][2 * g + 1] = v.y;
+        }
+        most = 255u;
     }
+    // Bytes above 252, which no append writes, count as 252 in a block with masked tokens: such
+    // a token's values stay finite.
+    __device__ __forceinline__ void bound() { most = 252u; }
+
+    // Scale of token t for the lane's elements of chunk n.
+    __device__ __forceinline__ float scale(int t, int n, bool whole) const {
+        const int m = threadIdx.x & 15;
+        const int byte = (t & 3) * 2 * NG + 4 * n;  // the chunk's first, a multiple of 2
+        uint32_t d = b[t >> 2][byte >> 2];
+        if (byte & 2)  // (then NG is odd, and four bytes may lie in two words)
+            d = n < NC ? __builtin_amdgcn_alignbyte(b[t >> 2][(byte >> 2) + 1], d, 2) : d >> 16;
+        const uint32_t e = (d >> (8 * (n < NC ? m >> 2 : m >> 3))) & 0xffu;
+        return __uint_as_float((whole ? e : min(e, most)) << 23);
+    }
+
+    struct Acc {
+        f4v o[NC][8], x[ODD ? 4 : 1];
+
+        __device__ __forceinline__ void clear() { each([](f4v &y) { y = f4v{0.f, 0.f, 0.f, 0.f}; }); }
+        __device__ __forceinline__ void scale(float f) { each([=](f4v &y) { y *= f; }); }
+        template <typename F> __device__ __forceinline__ void each(F &&f) {
+#pragma unroll
+            for (int n = 0; n < NC; ++n)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    f(o[n][j]);
+            if constexpr (ODD) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    f(x[j]);
+            }
+        }
+        template <int TP>
+        __device__ __forceinline__ void add(const Vals &v, const float (&p)[8], bool whole) {
+            bf16x8 b[TP];
+            split8<TP>(p, b);
+#pragma unroll
+            for (int n = 0; n < NC + ODD; ++n) {
+                float s[8];
+#pragma unroll
+                for (int t = 0; t < 8; ++t)
+                    s[t] = v.scale(t, n, whole);
+#pragma unroll
+                for (int z = 0; z < (n < NC ? 4 : 2); ++z) {  // byte z: elements 2 z and 2 z + 1
+                    bf16x8 a0, a1;
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        const uint32_t c = as_u32(cvt4(v.w[n][2 * h], s[2 * h], z));
+                        const uint32_t d = as_u32(cvt4(v.w[n][2 * h + 1], s[2 * h + 1], z));
+                        const bf16x2 lo = as_bf2(__builtin_amdgcn_perm(d, c, 0x05040100u));
+                        const bf16x2 hi = as_bf2(__builtin_amdgcn_perm(d, c, 0x07060302u));
+                        a0[2 * h] = lo[0]; a0[2 * h + 1] = lo[1];
+                        a1[2 * h] = hi[0]; a1[2 * h + 1] = hi[1];
+                    }
+                    f4v &y0 = n < NC ? o[n < NC ? n : 0][2 * z] : x[ODD ? (2 * z) & 3 : 0];
+                    f4v &y1 = n < NC ? o[n < NC ? n : 0][2 * z + 1] : x[ODD ? (2 * z + 1) & 3 : 0];
+#pragma unroll
+                    for (int k = TP - 1; k >= 0; --k) {
+                        y0 = mfma(a0, b[k], y0);
+                        y1 = mfma(a1, b[k], y1);
+                    }
+                }
+            }
+        }
+        static __device__ __forceinline__ bf16x2 cvt4(uint32_t w, float s, int z) {
+            return z == 0   ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0)
+                   : z == 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1)
+                   : z == 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2)
+                            : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3);
+        }
+        template <typename F> __device__ __forceinline__ void pieces(int kg, F &&f) const {
+#pragma unroll
+            for (int n = 0; n < NC; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int d = 128 * n + 32 * kg + 8 * i;
+                    f(d, make_float4(o[n][0][i], o[n][1][i], o[n][2][i], o[n][3][i]));
+                    f(d + 4, make_float4(o[n][4][i], o[n][5][i], o[n][6][i], o[n][7][i]));
+                }
+            if constexpr (ODD) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    f(128 * NC + 16 * kg + 4 * i, make_float4(x[0][i], x[1][i], x[2][i], x[3][i]));
+            }
+        }
+    };
+};
+
+__device__ __forceinline__ void store4(float *p, float4 y) { *reinterpret_cast<float4 *>(p) = y; }
+__device__ __forceinline__ void store4(__bf16 *p, float4 y) {
+    const bf16x2 a = {(__bf16)y.x, (__bf16)y.y}, b = {(__bf16)y.z, (__bf16)y.w};
+    *reinterpret_cast<uint2 *>(p) = make_uint2(as_u32(a), as_u32(b));
+}
+
+// Where 16 tokens from t0 on (a multiple of 16) lie: the pool page (-1: nowhere) and its slot.
+struct Place {
+    int phys, slot;
+};
+__device__ __forceinline__ Place place_of(const AttnArgs &A, const Tile &t, int t0) {
+    const int pg = kv4_page_of(A.c, t0);
+    return {__builtin_amdgcn_readfirstlane(kv4_phys(A.c, t.table, A.s.max_pages, pg)),
+            t0 - pg * A.c.page};
 }
 
 }  // namespace
 
-// One workgroup: 16 rows of one sequence and kv head over one split of the tokens; its four
-// waves take blocks of 32 tokens in turn and join at the end.  S^T = K q^T puts a row in a
-// column of the accumulator (lanes c, c + 16, ...), so the probabilities are already where
+// Waves a SIMD whose registers hold an attention kernel without spilling.
+constexpr int attn_waves(int fmt, int ng, bool f32) {
+    return ng <= 2 && !f32 && (ng == 1 || fmt == 7) ? 3 : ng <= 2 || (ng == 3 && fmt == 7) || (fmt == 7 && !f32) ? 2 : 1;
+}
+
+// One workgroup: tiles of 16 rows of one sequence and kv head over one split of the tokens;
+// its four waves take blocks of 32 tokens in turn and join at the end.  S^T = K q^T puts a row
+// in a column of the accumulator (lanes c, c + 16, ...), so the probabilities are already where
 // the second product O^T = V^T P^T wants its right operand: token order inside a product is
-// free, and the value loads follow it.
+// free, and the value loads follow it.  Codes go from memory to the operands in registers.
+//
+// Each wave asks for the next block's keys as soon as it is done with this one's, so they are
+// on their way during the exponentials and the second product, and for its values after that:
+// what bounds the kernel is how many bytes are on their way.  (Two whole blocks in registers
+// halve the waves that fit.)  The pool pages are looked up one block earlier.  The maximum is
+// raised only when a block passes it by 2^8 (sums stay in range, and relative precision does
+// not depend on it), so most blocks need no exchange between lanes and no rescaling.
 template <int FMT, int NG, typename T>
-__global__ __launch_bounds__(256) void k_kv4_attn(AttnArgs A) {
+__global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv4_attn(AttnArgs A) {
     constexpr int D = 64 * NG, TQ = sizeof(T) == 4 ? 3 : 1, TP = sizeof(T) == 4 ? 3 : 2;
+    using V = Vals<FMT, NG, TP == 2>;
     __shared__ __attribute__((aligned(16))) float osum[3][16][D + 4];
     __shared__ float wm[4][16], wl[4][16];
     const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
@@ -261,157 +464,159 @@ __global__ __launch_bounds__(256) void k_kv4_attn(AttnArgs A) {
     const int split = blockIdx.x % A.splits;
     const Tile t = tile_of(A, blockIdx.z, blockIdx.y);
     for (int r0 = blockIdx.x / A.splits * 16; r0 < t.rows; r0 += A.tiles * 16) {
-    const int r1 = min(t.rows, r0 + 16);
-    int lo, hi;
-    span_of(A, t, r0, r1, lo, hi);
-    const int s0 = max(lo & ~31, split * A.chunk);
-    const int s1 = split + 1 == A.splits ? hi : min(hi, (split + 1) * A.chunk);
-    const int row = r0 + col;
-    const bool live = row < r1;
-    const int pos = t.pos0 + (live ? row : r0) / A.group;
-    const int from = A.window > 0 ? pos - A.window : -1;  // sees tokens above `from`
+        const int r1 = min(t.rows, r0 + 16);
+        int lo, hi;
+        span_of(A, t, r0, r1, lo, hi);
+        const int s0 = max(lo & ~31, split * A.chunk);
+        const int s1 = split + 1 == A.splits ? hi : min(hi, (split + 1) * A.chunk);
+        const int row = r0 + col;
+        const bool live = row < r1;
+        const int pos = t.pos0 + (live ? row : r0) / A.group;
+        const int from = A.window > 0 ? pos - A.window : -1;  // sees tokens above `from`
+        // tokens that every row of the tile sees: [all0, all1)
+        const int all1 = min(s1, t.pos0 + r0 / A.group + 1);
+        const int all0 = A.window > 0 ? t.pos0 + (r1 - 1) / A.group - A.window + 1 : 0;
 
-    bf16x8 q[NG][2][TQ];
-    load_q<FMT, NG, TQ, T>(A, t, row, live, q);
-    f4v o[NG][4];
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            o[g][j] = f4v{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
-
-    for (int t0 = s0 + 32 * wave; t0 < s1; t0 += 128) {
+        Place at[2], ahead[2];
         Keys<FMT, NG> k[2];
-        Vals<FMT, NG> v;
-        bool ok[2];
+        V v;
+        auto look = [&](int t0) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int tt = t0 + 16 * h, pg = kv4_page_of(A.c, tt);
-            const int phys = __builtin_amdgcn_readfirstlane(
-                kv4_phys(A.c, t.table, A.s.max_pages, pg));
-            ok[h] = phys >= 0;  // a page that is none: its tokens are not there
-            const size_t r = kv4_row(A.c, max(phys, 0), t.head, tt - pg * A.c.page);
-            k[h].load(A.c, r);
-            v.load(A.c, r, h);
+            for (int h = 0; h < 2; ++h)
+                ahead[h] = place_of(A, t, t0 + 16 * h);
+        };
+        auto fetch_keys = [&] {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                k[h].load(A.c, kv4_row(A.c, max(at[h].phys, 0), t.head, at[h].slot));
+        };
+        auto fetch_vals = [&] {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                v.load(A.c, kv4_row(A.c, max(at[h].phys, 0), t.head, at[h].slot), h);
+        };
+        const int b0 = s0 + 32 * wave;
+        if (b0 < s1) {
+            look(b0);
+            at[0] = ahead[0];
+            at[1] = ahead[1];
+            fetch_keys();
+            fetch_vals();
+            look(b0 + 128);
         }
-        float p[8], top = m;
-        uint32_t seen = 0;
+        bf16x8 q[NG][2][TQ];
+        load_q<FMT, NG, TQ, T>(A, t, row, live, q);
+        float k8[NG];  // what the codes' offset of 8 adds to a sum of products
+        if constexpr (FMT == 4)
+            offsets_of<NG, TQ>(q, k8);
+        typename V::Acc o;
+        o.clear();
+        float m = -INFINITY, l = 0.f;
+
+        for (int t0 = b0; t0 < s1; t0 += 128) {
+            // a page that is none: its tokens are not there
+            const bool ok[2] = {at[0].phys >= 0, at[1].phys >= 0};
+            const bool more = t0 + 128 < s1;
+            float p[8], top = -INFINITY;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const f4v s = dot_keys<FMT, NG, TQ>(k[h], q);
+            for (int h = 0; h < 2; ++h) {
+                const f4v s = dot_keys<FMT, NG, TQ>(k[h], q, k8);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int tok = t0 + 16 * h + 4 * kg + i;
-                const bool sees = ok[h] && live && tok < s1 && tok <= pos && tok > from;
-                p[4 * h + i] = s[i];
-                seen |= (uint32_t)sees << (4 * h + i);
-                top = fmaxf(top, sees ? s[i] * A.scale2 : -INFINITY);
+                for (int i = 0; i < 4; ++i)
+                    p[4 * h + i] = s[i];
             }
-        }
-        top = col_max(top);
-        const float ref = top == -INFINITY ? 0.f : top;
-        const float fix = __builtin_amdgcn_exp2f(m - ref);
-        m = top;
-        l *= fix;
+            if (more) {
+                at[0] = ahead[0];
+                at[1] = ahead[1];
+                fetch_keys();
+                look(t0 + 256);
+            }
+            const bool whole = ok[0] && ok[1] && t0 >= all0 && t0 + 32 <= all1;
+            uint32_t seen = 0xffu;
+            if (!whole) {
+                seen = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            p[i] = (seen >> i) & 1 ? power<T>(A, p[i], ref) : 0.f;
-            l += p[i];
-        }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            bf16x8 a[4], b[TP];
-            decode_vals<FMT, NG>(v, g, a);
-            if constexpr (FMT == 4) {
-                float ps[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i)  // a masked token's scale may be anything
-                    ps[i] = p[i] == 0.f ? 0.f : p[i] * v.s[i * NG + g];
-                split8<TP>(ps, b);
+                for (int i = 0; i < 8; ++i) {
+                    const int tok = t0 + 16 * (i >> 2) + 4 * kg + (i & 3);
+                    const bool sees = ok[i >> 2] && live && tok < s1 && tok <= pos && tok > from;
+                    seen |= (uint32_t)sees << i;
+                    top = fmaxf(top, sees ? p[i] * A.scale2 : -INFINITY);
+                }
+                v.bound();
             } else {
-                split8<TP>(p, b);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    top = fmaxf(top, p[i] * A.scale2);
             }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                o[g][j] *= fix;
-#pragma unroll
-                for (int k = TP - 1; k >= 0; --k)
-                    o[g][j] = mfma(a[j], b[k], o[g][j]);
+            if (__any(top > m + 8.f)) {
+                top = fmaxf(m, col_max(top));
+                const float fix = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
+                m = top;
+                l *= fix;
+                o.scale(fix);
             }
-        }
-    }
-    // join the waves: each one's sums relative to the common maximum
-    l = col_sum(l);
-    if (kg == 0) {
-        wm[wave][col] = m;
-        wl[wave][col] = l;
-    }
-    __syncthreads();
-    float M = wm[0][col], L = 0.f;
+            const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int w = 1; w < 4; ++w)
-        M = fmaxf(M, wm[w][col]);
-    const float ref = M == -INFINITY ? 0.f : M;
+            for (int i = 0; i < 8; ++i)
+                p[i] = power<T>(A, p[i], ref);
+            if (!whole) {
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
-        L += wl[w][col] * __builtin_amdgcn_exp2f(wm[w][col] - ref);
-    const float fix = __builtin_amdgcn_exp2f(m - ref);
-    if (wave > 0) {
-#pragma unroll
-        for (int g = 0; g < NG; ++g)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)  // lane: elements 64 g + 16 kg + 4 i + j
-                *reinterpret_cast<float4 *>(&osum[wave - 1][col][64 * g + 16 * kg + 4 * i]) =
-                    make_float4(o[g][0][i] * fix, o[g][1][i] * fix, o[g][2][i] * fix,
-                                o[g][3][i] * fix);
-    }
-    __syncthreads();
-    if (wave == 0 && live) {
-    const int tok = t.first + row / A.group, head = t.head * A.group + row % A.group;
-    const size_t at = ((size_t)split * A.s.n_tok + tok) * A.n_q + head;
-    if (A.splits > 1) {
-        if (kg == 0)
-            A.ml[at] = make_float2(M, L);
-    } else if (A.lse && kg == 0) {
-        A.lse[at] = L > 0.f ? M + log2f(L) : -INFINITY;
-    }
-    // (the joining kernel leaves a part of nothing out)
-    const float scale = A.splits > 1 ? 1.f : L > 0.f || L != L ? 1.f / L : 0.f;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-        float x[16];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float4 y = make_float4(o[g][0][i] * fix, o[g][1][i] * fix, o[g][2][i] * fix,
-                                   o[g][3][i] * fix);
-#pragma unroll
-            for (int w = 0; w < 3; ++w) {
-                const float4 z =
-                    *reinterpret_cast<const float4 *>(&osum[w][col][64 * g + 16 * kg + 4 * i]);
-                y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+                for (int i = 0; i < 8; ++i)
+                    p[i] = (seen >> i) & 1 ? p[i] : 0.f;
             }
-            x[4 * i] = y.x * scale; x[4 * i + 1] = y.y * scale;
-            x[4 * i + 2] = y.z * scale; x[4 * i + 3] = y.w * scale;
+            l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            o.template add<TP>(v, p, whole);
+            if (more)
+                fetch_vals();
         }
-        const int d = 64 * g + 16 * kg;
-        float x0[8], x1[8];
+        // join the waves: each one's sums relative to the common maximum
+        l = col_sum(l);
+        if (kg == 0) {
+            wm[wave][col] = m;
+            wl[wave][col] = l;
+        }
+        __syncthreads();
+        float M = wm[0][col], L = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            x0[i] = x[i];
-            x1[i] = x[8 + i];
+        for (int w = 1; w < 4; ++w)
+            M = fmaxf(M, wm[w][col]);
+        const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+            L += wl[w][col] * __builtin_amdgcn_exp2f(wm[w][col] - ref);
+        const float fix = __builtin_amdgcn_exp2f(m - ref);
+        if (wave > 0) {
+            o.pieces(kg, [&](int d, float4 y) {
+                *reinterpret_cast<float4 *>(&osum[wave - 1][col][d]) =
+                    make_float4(y.x * fix, y.y * fix, y.z * fix, y.w * fix);
+            });
         }
-        if (A.splits > 1) {
-            Vec8<float>::store(A.part + at * D + d, x0);
-            Vec8<float>::store(A.part + at * D + d + 8, x1);
-        } else {
-            T *out = static_cast<T *>(A.out) + ((size_t)tok * A.n_q + head) * D + d;
-            Vec8<T>::store(out, x0);
-            Vec8<T>::store(out + 8, x1);
+        __syncthreads();
+        if (wave == 0 && live) {
+            const int tok = t.first + row / A.group, head = t.head * A.group + row % A.group;
+            const size_t at = ((size_t)split * A.s.n_tok + tok) * A.n_q + head;
+            if (A.splits > 1) {
+                if (kg == 0)
+                    A.ml[at] = make_float2(M, L);
+            } else if (A.lse && kg == 0) {
+                A.lse[at] = L > 0.f ? M + log2f(L) : -INFINITY;
+            }
+            const float scale = A.splits > 1 ? 1.f : L > 0.f || L != L ? 1.f / L : 0.f;
+            o.pieces(kg, [&](int d, float4 y) {
+                y = make_float4(y.x * fix, y.y * fix, y.z * fix, y.w * fix);
+#pragma unroll
+                for (int w = 0; w < 3; ++w) {
+                    const float4 z = *reinterpret_cast<const float4 *>(&osum[w][col][d]);
+                    y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+                }
+                y = make_float4(y.x * scale, y.y * scale, y.z * scale, y.w * scale);
+                if (A.splits > 1)
+                    *reinterpret_cast<float4 *>(A.part + at * D + d) = y;
+                else
+                    store4(static_cast<T *>(A.out) + ((size_t)tok * A.n_q + head) * D + d, y);
+            });
         }
-    }
-    }
-    __syncthreads();
+        __syncthreads();
     }
 }
 
@@ -495,9 +700,12 @@ __global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs A) {
                      : -INFINITY;
             bf16x8 q[NG][2][TQ];
             load_q<FMT, NG, TQ, T>(A, t, row, live, q);
+            float k8[NG];
+            if constexpr (FMT == 4)
+                offsets_of<NG, TQ>(q, k8);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const f4v s = dot_keys<FMT, NG, TQ>(k[h], q);
+                const f4v s = dot_keys<FMT, NG, TQ>(k[h], q, k8);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int tok = t0 + 16 * h + 4 * kg + i;

@@ -225,7 +225,7 @@ __global__ __launch_bounds__(256) void k_kv4_append(Kv4View C, Kv4Seqs S, const 
     uint8_t *sc = isv ? C.vs : C.ks;
     if constexpr (FMT == 4) {
         const bool tiny = top < kKv4Tiny;
-        const float s = tiny ? 0.f : top / 7.f, inv = tiny ? 0.f : 1.f / s;
+        const float s = tiny ? 0.f : top * (1.f / 7.f), inv = tiny ? 0.f : 1.f / s;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             codes |= (uint32_t)(tiny ? 8 : kv4_round(x[i], s, inv) + 8) << (4 * i);

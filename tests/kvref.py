@@ -35,7 +35,7 @@ def quantize(fmt, x):
     g = x.reshape(*x.shape[:-1], -1, GROUP[fmt])
     top = np.abs(g).max(-1)
     if fmt == 4:
-        s = np.where(top < TINY, 0.0, (top.astype(np.float32) / np.float32(7)).astype(np.float64))
+        s = np.where(top < TINY, 0.0, (top.astype(np.float32) * np.float32(1 / 7)).astype(np.float64))
         n = np.where(s[..., None] > 0, np.rint(g / np.where(s > 0, s, 1)[..., None]), 0).clip(-7, 7)
         n, s = n.astype(np.int64) + 8, s.astype(np.float32)
     else:

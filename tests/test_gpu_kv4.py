@@ -177,7 +177,7 @@ def test_append_rounds_exactly(hip, fmt):
     rng = np.random.default_rng(fmt)
     T, D = 600, 64
     top = np.exp(rng.uniform(-60, 60, (T, 1))).astype(np.float32)
-    s = top / np.float32(7) if fmt == 4 else np.float32(2.0) ** np.ceil(np.log2(top / 6))
+    s = top * np.float32(1 / 7) if fmt == 4 else np.float32(2.0) ** np.ceil(np.log2(top / 6))
     mids = np.arange(-6.5, 7) if fmt == 4 else \
         np.concatenate(((kvref.GRID[1:] + kvref.GRID[:-1]) / 2, -(kvref.GRID[1:] + kvref.GRID[:-1]) / 2))
     x = (np.resize(mids, (T, D)) * s.astype(np.float64)).astype(np.float32)
