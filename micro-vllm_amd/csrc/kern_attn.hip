@@ -37,7 +37,8 @@ template <typename T> __device__ __forceinline__ float power(const AttnArgs &A, 
     return __builtin_amdgcn_exp2f(fmaf(s, A.scale2, -ref));
 }
 
-// x[8] as T bf16 operands that add up to it (T = 3: all 24 bits).
+// x[8] as T bf16 operands that add up to it (T = 3: all 24 bits).  An infinite x becomes NaN,
+// as does every row that an infinite query or probability is in.
 template <int T>
 __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&t)[T]) {
 #pragma unroll
@@ -47,7 +48,7 @@ __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&t)[T]) {
         for (int k = 0; k < T; ++k) {
             t[k][i] = (__bf16)r;
             if (k + 1 < T)
-                r = nonfinite((float)t[k][i]) ? 0.f : r - (float)t[k][i];
+                r -= (float)t[k][i];
         }
     }
 }
@@ -84,27 +85,33 @@ __device__ __forceinline__ void span_of(const AttnArgs &A, const Tile &t, int r0
 }
 
 // B operands of 16 rows of queries: lane (column c, group of lanes kg) holds, of each 64
-// elements g, the 16 from 64 g + 16 kg, as two operands (int4: in decode_b<4>'s order).
+// elements g, the 16 from 64 g + 16 kg, as two operands (int4: in decode_b<4>'s order).  k8: -8
+// times a row's sum of queries in each group, from which the sums of products with int4 codes n
+// start, so that they end as those with n - 8 (one instruction for 4 codes in place of five).
 template <int FMT, int NG, int TQ, typename T>
 __device__ __forceinline__ void load_q(const AttnArgs &A, const Tile &t, int row, bool live,
-                                       bf16x8 (&q)[NG][2][TQ]) {
+                                       bf16x8 (&q)[NG][2][TQ], float (&k8)[NG]) {
     const int kg = (threadIdx.x & 63) >> 4;
     const int tok = t.first + (live ? row / A.group : 0);
     const int head = t.head * A.group + (live ? row % A.group : 0);
     const T *p = static_cast<const T *>(A.q) + (size_t)tok * A.q_stride +
                  (size_t)head * (64 * NG) + 16 * kg;
 #pragma unroll
-    for (int g = 0; g < NG; ++g)
+    for (int g = 0; g < NG; ++g) {
+        float sum = 0.f;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, y[8];
             if (live)
                 Vec8<T>::load(p + 64 * g + 8 * s, x);
+            sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 y[a_slot<FMT>(e)] = x[e];
             split8<TQ>(y, q[g][s]);
         }
+        k8[g] = FMT == 4 ? -8.f * col_sum(sum) : 0.f;
+    }
 }
 
 // 16 tokens' keys as the lanes need them: lane (token m, kg) codes of the 16 elements from
@@ -135,25 +142,6 @@ template <int FMT, int NG> struct Keys {
         }
     }
 };
-
-// -8 times each row's sum of queries in each group of 64: what the sums of products with int4
-// codes n start from, so that they end as those with n - 8 (one instruction for 4 codes in place
-// of five).
-template <int NG, int TQ>
-__device__ __forceinline__ void offsets_of(const bf16x8 (&q)[NG][2][TQ], float (&k8)[NG]) {
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-        float sum = 0.f;
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int k = TQ - 1; k >= 0; --k)
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    sum += (float)q[g][s][k][e];
-        k8[g] = -8.f * col_sum(sum);
-    }
-}
 
 // Products of 16 tokens' keys with 16 rows of queries: S[i] is token 4 kg + i, row c.  An int4
 // group's codes are summed exactly and its scale applied to the sum; an MXFP4 code times its
@@ -214,7 +202,14 @@ template <int NG, bool UNS> struct Vals<4, NG, UNS> {
             s[o] = v.x; s[o + 1] = v.y; s[o + 2] = v.z; s[o + 3] = v.w;
         }
     }
-    __device__ __forceinline__ void bound() {}  // add() leaves a masked token's scale out
+    // A masked token's scale may be anything: the lane's row takes none.
+    __device__ __forceinline__ void hide(uint32_t seen) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+                s[i * NG + g] = (seen >> i) & 1 ? s[i * NG + g] : 0.f;
+    }
 
     struct Acc {
         f4v o[NG][4], e[NG];
@@ -238,7 +233,7 @@ template <int NG, bool UNS> struct Vals<4, NG, UNS> {
             }
         }
         template <int TP>
-        __device__ __forceinline__ void add(const Vals &v, const float (&p)[8], bool whole) {
+        __device__ __forceinline__ void add(const Vals &v, const float (&p)[8]) {
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 float ps[8];
@@ -246,11 +241,6 @@ template <int NG, bool UNS> struct Vals<4, NG, UNS> {
                 for (int i = 0; i < 8; ++i)
                     ps[i] = p[i] * v.s[i * NG + g];
                 __builtin_amdgcn_sched_barrier(0);  // one group's operands at a time
-                if (!whole) {  // a masked token's scale may be anything
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        ps[i] = p[i] == 0.f ? 0.f : ps[i];
-                }
                 bf16x8 b[TP], a[4];
                 split8<TP>(ps, b);
 #pragma unroll
@@ -305,7 +295,6 @@ template <int NG, bool UNS> struct Vals<7, NG, UNS> {
     static constexpr int NC = NG / 2, ODD = NG & 1;
     uint32_t w[NC + ODD][8];
     uint32_t b[2][2 * NG];  // scale bytes [token][2 NG] of 4 tokens
-    uint32_t most;          // largest scale byte that counts
 
     __device__ __forceinline__ void load(const Kv4View &c, size_t row, int half) {
         const int lane = threadIdx.x & 63, m = lane & 15, kg = lane >> 4;
@@ -328,21 +317,29 @@ template <int NG, bool UNS> struct Vals<7, NG, UNS> {
             b[half][2 * g] = v.x;
             b[half][2 * g + 1] = v.y;
         }
-        most = 255u;
     }
     // Bytes above 252, which no append writes, count as 252 in a block with masked tokens: such
     // a token's values stay finite.
-    __device__ __forceinline__ void bound() { most = 252u; }
+    __device__ __forceinline__ void hide(uint32_t) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 2 * NG; ++i) {
+                const uint32_t x = b[h][i];
+                b[h][i] = min(x & 0xffu, 252u) | min(x & 0xff00u, 252u << 8) |
+                          min(x & 0xff0000u, 252u << 16) | min(x & 0xff000000u, 252u << 24);
+            }
+    }
 
     // Scale of token t for the lane's elements of chunk n.
-    __device__ __forceinline__ float scale(int t, int n, bool whole) const {
+    __device__ __forceinline__ float scale(int t, int n) const {
         const int m = threadIdx.x & 15;
         const int byte = (t & 3) * 2 * NG + 4 * n;  // the chunk's first, a multiple of 2
         uint32_t d = b[t >> 2][byte >> 2];
         if (byte & 2)  // (then NG is odd, and four bytes may lie in two words)
             d = n < NC ? __builtin_amdgcn_alignbyte(b[t >> 2][(byte >> 2) + 1], d, 2) : d >> 16;
         const uint32_t e = (d >> (8 * (n < NC ? m >> 2 : m >> 3))) & 0xffu;
-        return __uint_as_float((whole ? e : min(e, most)) << 23);
+        return __uint_as_float(e << 23);
     }
 
     struct Acc {
@@ -363,7 +360,7 @@ template <int NG, bool UNS> struct Vals<7, NG, UNS> {
             }
         }
         template <int TP>
-        __device__ __forceinline__ void add(const Vals &v, const float (&p)[8], bool whole) {
+        __device__ __forceinline__ void add(const Vals &v, const float (&p)[8]) {
             bf16x8 b[TP];
             split8<TP>(p, b);
 #pragma unroll
@@ -371,7 +368,7 @@ template <int NG, bool UNS> struct Vals<7, NG, UNS> {
                 float s[8];
 #pragma unroll
                 for (int t = 0; t < 8; ++t)
-                    s[t] = v.scale(t, n, whole);
+                    s[t] = v.scale(t, n);
 #pragma unroll
                 for (int z = 0; z < (n < NC ? 4 : 2); ++z) {  // byte z: elements 2 z and 2 z + 1
                     bf16x8 a0, a1;
@@ -461,9 +458,9 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
     __shared__ float wm[4][16], wl[4][16];
     const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int split = blockIdx.x % A.splits;
-    const Tile t = tile_of(A, blockIdx.z, blockIdx.y);
-    for (int r0 = blockIdx.x / A.splits * 16; r0 < t.rows; r0 += A.tiles * 16) {
+    const int split = blockIdx.z % A.splits;
+    const Tile t = tile_of(A, blockIdx.y, blockIdx.x);
+    for (int r0 = blockIdx.z / A.splits * 16; r0 < t.rows; r0 += A.tiles * 16) {
         const int r1 = min(t.rows, r0 + 16);
         int lo, hi;
         span_of(A, t, r0, r1, lo, hi);
@@ -505,10 +502,8 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
             look(b0 + 128);
         }
         bf16x8 q[NG][2][TQ];
-        load_q<FMT, NG, TQ, T>(A, t, row, live, q);
-        float k8[NG];  // what the codes' offset of 8 adds to a sum of products
-        if constexpr (FMT == 4)
-            offsets_of<NG, TQ>(q, k8);
+        float k8[NG];
+        load_q<FMT, NG, TQ, T>(A, t, row, live, q, k8);
         typename V::Acc o;
         o.clear();
         float m = -INFINITY, l = 0.f;
@@ -517,13 +512,15 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
             // a page that is none: its tokens are not there
             const bool ok[2] = {at[0].phys >= 0, at[1].phys >= 0};
             const bool more = t0 + 128 < s1;
-            float p[8], top = -INFINITY;
+            float s[8], x[8], p[8];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const f4v s = dot_keys<FMT, NG, TQ>(k[h], q, k8);
+                const f4v y = dot_keys<FMT, NG, TQ>(k[h], q, k8);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    p[4 * h + i] = s[i];
+                for (int i = 0; i < 4; ++i) {
+                    s[4 * h + i] = y[i];
+                    x[4 * h + i] = y[i] * A.scale2;
+                }
             }
             if (more) {
                 at[0] = ahead[0];
@@ -531,41 +528,34 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
                 fetch_keys();
                 look(t0 + 256);
             }
-            const bool whole = ok[0] && ok[1] && t0 >= all0 && t0 + 32 <= all1;
-            uint32_t seen = 0xffu;
-            if (!whole) {
-                seen = 0;
+            if (!(ok[0] && ok[1] && t0 >= all0 && t0 + 32 <= all1)) {
+                uint32_t seen = 0;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int tok = t0 + 16 * (i >> 2) + 4 * kg + (i & 3);
                     const bool sees = ok[i >> 2] && live && tok < s1 && tok <= pos && tok > from;
                     seen |= (uint32_t)sees << i;
-                    top = fmaxf(top, sees ? p[i] * A.scale2 : -INFINITY);
+                    x[i] = sees ? x[i] : -INFINITY;
                 }
-                v.bound();
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    top = fmaxf(top, p[i] * A.scale2);
+                v.hide(seen);
             }
+            const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                                    fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
             if (__any(top > m + 8.f)) {
-                top = fmaxf(m, col_max(top));
-                const float fix = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
-                m = top;
+                const float up = fmaxf(m, col_max(top));
+                const float fix = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - up);
+                m = up;
                 l *= fix;
                 o.scale(fix);
             }
             const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                p[i] = power<T>(A, p[i], ref);
-            if (!whole) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    p[i] = (seen >> i) & 1 ? p[i] : 0.f;
-            }
+                p[i] = sizeof(T) == 2       ? __builtin_amdgcn_exp2f(x[i] - ref)
+                       : x[i] == -INFINITY ? 0.f
+                                            : power<T>(A, s[i], ref);
             l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-            o.template add<TP>(v, p, whole);
+            o.template add<TP>(v, p);
             if (more)
                 fetch_vals();
         }
@@ -602,6 +592,7 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
                 A.lse[at] = L > 0.f ? M + log2f(L) : -INFINITY;
             }
             const float scale = A.splits > 1 ? 1.f : L > 0.f || L != L ? 1.f / L : 0.f;
+            if (A.splits == 1 || M != -INFINITY)  // (the join leaves a split of nothing out)
             o.pieces(kg, [&](int d, float4 y) {
                 y = make_float4(y.x * fix, y.y * fix, y.z * fix, y.w * fix);
 #pragma unroll
@@ -620,42 +611,63 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
     }
 }
 
-// Joins the splits of the rows that belong to a sequence: one workgroup of D / 8 lanes a head,
-// 256 / (D / 8) heads of one token.
+// Joins the splits of the rows that belong to a sequence.  One wave a head of a token: lane s
+// holds split s's maximum and sum (at most 64 splits), and groups of D / 8 lanes take every
+// other split's sums.
 template <int NG, typename T>
 __global__ __launch_bounds__(256) void k_kv4_join(AttnArgs A) {
-    constexpr int D = 64 * NG, LPH = D / 8, HPG = 256 / LPH;
-    const int tok = blockIdx.x, hi = threadIdx.x / LPH, d = (threadIdx.x % LPH) * 8;
-    const int head = blockIdx.y * HPG + hi;
-    if (hi >= HPG || head >= A.n_q)
-        return;
-    if (tok < A.s.q_start[0] || tok >= A.s.q_start[A.s.n_seq])
+    constexpr int D = 64 * NG, LPH = D / 8, G = 64 / LPH;
+    const int lane = threadIdx.x & 63;
+    const int tok = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 6);
+    if (head >= A.n_q || tok < A.s.q_start[0] || tok >= A.s.q_start[A.s.n_seq])
         return;
     const size_t at = (size_t)tok * A.n_q + head, step = (size_t)A.s.n_tok * A.n_q;
-    float M = -INFINITY;
-    for (int s = 0; s < A.splits; ++s)
-        M = fmaxf(M, A.ml[at + s * step].x);
-    float L = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < A.splits; ++s) {
-        const float2 ml = A.ml[at + s * step];
-        if (ml.x == -INFINITY) {
-            L += ml.y;  // 0, or NaN
-            continue;
-        }
-        const float f = __builtin_amdgcn_exp2f(ml.x - M);
-        float y[8];
-        Vec8<float>::load(A.part + (at + s * step) * D + d, y);
-        L = fmaf(ml.y, f, L);
+    const float2 ml = lane < A.splits ? A.ml[at + lane * step] : make_float2(-INFINITY, 0.f);
+    float M = ml.x;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            x[i] = fmaf(y[i], f, x[i]);
+    for (int o = 32; o >= 1; o >>= 1)
+        M = fmaxf(M, __shfl_xor(M, o));
+    const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - M);
+    float L = ml.y * f;  // a split of nothing: 0 (or NaN, which stays)
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1)
+        L += __shfl_xor(L, o);
+    const int g = lane / LPH, d = (lane - g * LPH) * 8;
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < A.splits; s0 += 4 * G) {
+        float y[4][8], w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {  // four loads on their way
+            const int s = min(s0 + u * G + g, 63);
+            const float has = __shfl(ml.x, s);
+            w[u] = __shfl(f, s);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                y[u][i] = 0.f;
+            if (g < G && has != -INFINITY)  // splits from A.splits on have none
+                Vec8<float>::load(A.part + (at + s * step) * D + d, y[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                x[i] = fmaf(y[u][i], w[u], x[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float sum = x[i];
+#pragma unroll
+        for (int n = 1; n < G; ++n)
+            sum += __shfl(x[i], (lane + n * LPH) & 63);
+        x[i] = sum;
     }
     const float scale = L > 0.f || L != L ? 1.f / L : 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         x[i] *= scale;
-    Vec8<T>::store(static_cast<T *>(A.out) + at * D + d, x);
-    if (A.lse && d == 0)
+    if (g == 0)
+        Vec8<T>::store(static_cast<T *>(A.out) + at * D + d, x);
+    if (A.lse && lane == 0)
         A.lse[at] = L > 0.f ? M + log2f(L) : -INFINITY;
 }
 
@@ -699,10 +711,8 @@ __global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs A) {
                              row % A.group]
                      : -INFINITY;
             bf16x8 q[NG][2][TQ];
-            load_q<FMT, NG, TQ, T>(A, t, row, live, q);
             float k8[NG];
-            if constexpr (FMT == 4)
-                offsets_of<NG, TQ>(q, k8);
+            load_q<FMT, NG, TQ, T>(A, t, row, live, q, k8);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const f4v s = dot_keys<FMT, NG, TQ>(k[h], q, k8);
@@ -733,14 +743,26 @@ __global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs A) {
     }
 }
 
-AttnPlan kv4_attention_plan(int head_dim, int n_kv, int n_q, int n_tok, int n_seq, int max_new,
-                            int max_len, bool weights) {
+// How a call is cut.  Up to 48 rows a sequence and kv head take the 16-row kernel, more the
+// kernel of kern_prompt.hip, with 8 waves (256 rows) a workgroup where that fills the chip.
+//
+// Splits of the tokens: enough workgroups to fill the chip (`fill`), but chunks of 128 tokens
+// (one block a wave) at least, and at most the 64 splits that a wave joins.  A workgroup's
+// start and end cost about as much as three blocks, so where registers allow two workgroups a
+// CU anyway, three times the CUs are best (768: 16 f32 int4 streams to 4096 tokens 54 us, 58 with
+// 2048, 62 with 512); bf16 over MXFP4, three a CU and less work a block, gains by finer chunks
+// (32 streams to 16384 tokens 110 us with 2048, 120 with 768).
+AttnPlan kv4_attention_plan(int fmt, int dtype, int head_dim, int n_kv, int n_q, int n_tok,
+                            int n_seq, int max_new, int max_len, bool weights) {
     AttnPlan p{};
-    const long long rows = (long long)max_new * (n_q / n_kv);
-    p.tiles = (int)((rows + 15) / 16);
-    const long long base = (long long)p.tiles * n_kv * n_seq;
-    const long long want = std::max(1ll, 1024 / base);
-    p.chunk = (int)std::max(256ll, ((max_len + want - 1) / want + 127) / 128 * 128);
+    const long long rows = (long long)max_new * (n_q / n_kv), pairs = (long long)n_kv * n_seq;
+    if (rows > 48)
+        p.waves = head_dim <= 128 && (rows + 255) / 256 * pairs >= 192 ? 8 : 4;
+    const int tile = p.waves ? 32 * p.waves : 16, least = p.waves ? 512 : 128;
+    const int fill = p.waves ? 256 : fmt == 7 && dtype == KV4_BF16 ? 2048 : 768;
+    p.tiles = (int)std::min(32768ll, (rows + tile - 1) / tile);
+    const long long want = std::max(1ll, std::min(64ll, fill / (p.tiles * pairs)));
+    p.chunk = (int)std::max((long long)least, ((max_len + want - 1) / want + 127) / 128 * 128);
     p.splits = (max_len + p.chunk - 1) / p.chunk;
     auto add = [&](size_t bytes) {
         const size_t at = p.bytes;
@@ -757,18 +779,36 @@ AttnPlan kv4_attention_plan(int head_dim, int n_kv, int n_q, int n_tok, int n_se
     return p;
 }
 
+size_t kv4_attention_bytes(int head_dim, int n_kv, int n_q, int n_tok, int n_seq, int max_new,
+                           int max_len, bool weights) {
+    size_t most = 0;
+    for (int fmt : {4, 7})
+        for (int dtype : {KV4_F32, KV4_BF16})
+            most = std::max(most, kv4_attention_plan(fmt, dtype, head_dim, n_kv, n_q, n_tok, n_seq,
+                                                     max_new, max_len, weights)
+                                      .bytes);
+    return most;
+}
+
 template <int FMT, int NG, typename T>
 static hipError_t attention(const AttnArgs &a, int max_len, hipStream_t st) {
-    const dim3 grid((unsigned)(a.splits * a.tiles), (unsigned)a.c.n_kv, (unsigned)a.s.n_seq);
+    hipError_t e;
+    if (a.waves) {
+        if ((e = launch_kv4_prompt(FMT, 64 * NG, sizeof(T) == 2 ? KV4_BF16 : KV4_F32, a.waves, a,
+                                   st)) != hipSuccess)
+            return e;
+    } else {
+    // Heads go round the XCDs first, splits last: sequences of unlike length leave the later
+    // splits empty, and with the splits first the XCDs that got those had nothing to do.
+    const dim3 grid((unsigned)a.c.n_kv, (unsigned)a.s.n_seq, (unsigned)(a.splits * a.tiles));
     hipLaunchKernelGGL((k_kv4_attn<FMT, NG, T>), grid, dim3(256), 0, st, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess)
+    if ((e = hipGetLastError()) != hipSuccess)
         return e;
+    }
     if (a.splits > 1) {
-        constexpr int HPG = 256 / (8 * NG);
         hipLaunchKernelGGL((k_kv4_join<NG, T>),
-                           dim3((unsigned)a.s.n_tok, (unsigned)((a.n_q + HPG - 1) / HPG)),
-                           dim3(256), 0, st, a);
+                           dim3((unsigned)a.s.n_tok, (unsigned)((a.n_q + 3) / 4)), dim3(256), 0,
+                           st, a);
         if ((e = hipGetLastError()) != hipSuccess)
             return e;
     }

@@ -235,9 +235,8 @@ long long mvllm_hip_kv4_attention_work(int n_kv, int head_dim, int n_q, int n_to
                                        int max_new, int max_len, int weights) {
     if (!attention_sizes_ok(head_dim, n_kv, n_q, n_tok, n_seq, max_new, max_len))
         return -1;
-    return (long long)kv4_attention_plan(head_dim, n_kv, n_q, n_tok, n_seq, max_new, max_len,
-                                         weights != KV4_WEIGHTS_NONE)
-        .bytes;
+    return (long long)kv4_attention_bytes(head_dim, n_kv, n_q, n_tok, n_seq, max_new, max_len,
+                                          weights != KV4_WEIGHTS_NONE);
 }
 
 int mvllm_hip_kv4_attention_dev(const mvllm_kv4 *cache, int dtype, const void *q,
@@ -265,10 +264,12 @@ int mvllm_hip_kv4_attention_dev(const mvllm_kv4 *cache, int dtype, const void *q
         (weights != KV4_WEIGHTS_NONE && !cache->score))
         return refuse("kv4_attention_dev: weights is 0, 1 or 2, and the cache has a score array "
                       "where it is not 0");
-    const AttnPlan p = kv4_attention_plan(D, a.c.n_kv, n_q, n_tok, n_seq, max_new, max_len,
-                                          weights != KV4_WEIGHTS_NONE);
-    if (p.bytes > work_bytes || (p.bytes && (!work || !aligned16(work))))
-        return refuse("kv4_attention_dev: the workspace needs " + std::to_string(p.bytes) +
+    const AttnPlan p = kv4_attention_plan(cache->fmt, dtype, D, a.c.n_kv, n_q, n_tok, n_seq,
+                                          max_new, max_len, weights != KV4_WEIGHTS_NONE);
+    const size_t need = kv4_attention_bytes(D, a.c.n_kv, n_q, n_tok, n_seq, max_new, max_len,
+                                            weights != KV4_WEIGHTS_NONE);
+    if (need > work_bytes || (need && (!work || !aligned16(work))))
+        return refuse("kv4_attention_dev: the workspace needs " + std::to_string(need) +
                       " bytes, 16-byte aligned (mvllm_hip_kv4_attention_work)");
     char *w = static_cast<char *>(work);
     a.q = q;
@@ -282,6 +283,7 @@ int mvllm_hip_kv4_attention_dev(const mvllm_kv4 *cache, int dtype, const void *q
     a.splits = p.splits;
     a.chunk = p.chunk;
     a.tiles = p.tiles;
+    a.waves = p.waves;
     const double scale2 = (double)scale * 1.44269504088896340736;
     a.scale2 = (float)scale2;
     a.scale2_lo = (float)(scale2 - (double)a.scale2);

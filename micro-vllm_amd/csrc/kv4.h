@@ -51,7 +51,7 @@ struct AttnArgs {
     float2 *ml;    // [splits][n_tok][n_q] maximum (log2) and sum of a split
     float *lse;    // [n_tok][n_q] log2 of a row's sum of exponentials (-inf: sees nothing), or null
     long long q_stride;
-    int n_q, group, splits, chunk, tiles;
+    int n_q, group, splits, chunk, tiles, waves;
     float scale2, scale2_lo;  // scale * log2(e), and what the f32 leaves of it
     int window, weights;
 };
@@ -74,11 +74,17 @@ hipError_t launch_kv4_evict(int fmt, int head_dim, const EvictArgs &a, int max_l
 
 // How a call is cut: the parts of its workspace follow from it.
 struct AttnPlan {
+    int waves;  // 0: 16 rows a workgroup, else 32 a wave
     int splits, chunk, tiles;
     size_t part, ml, lse, bytes;  // offsets into the workspace, and its size
 };
-AttnPlan kv4_attention_plan(int head_dim, int n_kv, int n_q, int n_tok, int n_seq, int max_new,
-                            int max_len, bool weights);
+AttnPlan kv4_attention_plan(int fmt, int dtype, int head_dim, int n_kv, int n_q, int n_tok,
+                            int n_seq, int max_new, int max_len, bool weights);
+// The workspace that serves every format and type.
+size_t kv4_attention_bytes(int head_dim, int n_kv, int n_q, int n_tok, int n_seq, int max_new,
+                           int max_len, bool weights);
+hipError_t launch_kv4_prompt(int fmt, int head_dim, int dtype, int waves, const AttnArgs &a,
+                             hipStream_t st);
 hipError_t launch_kv4_attention(int fmt, int head_dim, int dtype, const AttnArgs &a, int max_len,
                                 hipStream_t st);
 

@@ -77,13 +77,14 @@ def rows_of(q_start, lens):
 
 
 def attention(c, q, q_start, lens, table, scale, window, weights):
-    """-> out [T, Hq, D], mag (sum of P |v|), top (largest |log2 exponent|), score (or None);
-    rows of no sequence are NaN in out."""
+    """-> out [T, Hq, D], mag (sum of P |v|), sizes, score (or None); rows of no sequence are
+    NaN in out.  sizes, in log2 units of the exponents: the largest |exponent|, the largest sum of
+    |q k| and the largest root of the sum of (q k)^2."""
     T, Hq, D = q.shape
     Hkv = c["k"].shape[1]
     G = Hq // Hkv
     out, mag = np.full((T, Hq, D), np.nan), np.zeros((T, Hq, D))
-    top, err = 0.0, 0.0
+    top, err, err2 = 0.0, 0.0, 0.0
     score = c["score"].astype(np.float64) if weights else None
     for b in range(len(lens)):
         n = min(max(int(lens[b]), 0), table.shape[1] * c["page"])
@@ -114,10 +115,11 @@ def attention(c, q, q_start, lens, table, scale, window, weights):
                     if np.isfinite(s).all():
                         top = max(top, np.abs(s).max() * 1.4427)
                         err = max(err, (np.abs(k[sees]) @ np.abs(qr)).max() * abs(scale) * 1.4427)
+                        err2 = max(err2, np.sqrt((k[sees] ** 2 @ qr ** 2).max()) * abs(scale) * 1.4427)
             if weights:
                 old = score[pg[here], h, sl[here]]
                 score[pg[here], h, sl[here]] = got[here] + (old if weights == 1 else 0)
-    return out, mag, (top, err), score
+    return out, mag, (top, err, err2), score
 
 
 def evict(c, lens, table, keep, recent):

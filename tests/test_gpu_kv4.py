@@ -10,8 +10,15 @@ Bars, by the roundings that can meet (u = 2^-24, half an f32 step; h = 2^-8, hal
   of itself, a probability by ln 2 of that and 2 u, in numerator and denominator; the sums of n
   products add (n + 64) u of sum P |v|.  bf16: probabilities as two terms (h^2 / 2 of sum P |v|)
   and the output's own h.
+- attention of more than 48 rows of a kv head (f16 operands, f = 2^-12 half an f16 step): bf16
+  calls round a probability once (f), an int4 scale and its product with a code once each, of
+  keys (an exponent is off by 2 f of sum |q k|) and of values (2 f of sum P |v|); MXFP4 is exact.
+  f32 calls hold each rounded operand in two terms (f^2 of it, 2^-24, taken as 2 u for its
+  subnormal second terms) and leave out the product of the second two (f^2): 3 * 2 u of sum
+  |q k| and of sum P |v|.
 - the 2-norm: errors of independent roundings grow as their root: exponents 4 u of the largest
-  one, 16 u beside.
+  one, 16 u beside; f16 keys' 2 f of the root of the sum of (q k)^2, twice for the
+  denominator's share; f16 values and probabilities 3 f.
 - eviction: indices, codes, scales and scores equal.
 """
 import numpy as np
@@ -222,22 +229,26 @@ def run_attention(hip, cache, dtype, q, q_start, lens, tab, max_new, max_len, sc
 def check_attention(c, q, got, score, q_start, lens, tab, scale, window, weights, dtype,
                     fill=5.0):
     D = q.shape[2]
-    out, mag, (top, sums), exp_score = kvref.attention(c, q, q_start, lens, tab, scale, window,
-                                                       weights)
+    out, mag, (top, sums, root), exp_score = kvref.attention(c, q, q_start, lens, tab, scale,
+                                                             window, weights)
     own = ~np.isnan(out).all((1, 2))
     assert (got[~own] == fill).all()
-    p_off = 2 * (np.log(2) * U * (D * sums + 2 * top) + 2 * U)
-    tol = mag * (p_off + (max(max(lens), 1) + 64) * U)
+    prompt = int(np.max(np.diff(q_start))) * (q.shape[1] // c["k"].shape[1]) > 48
+    f = 2.0 ** -12 if prompt else 0.0
+    k_off = (2 * f if c["fmt"] == 4 else 0) if dtype == "bf16" else 6 * U * prompt
+    v_off = (3 * f if c["fmt"] == 4 else f) if dtype == "bf16" else 6 * U * prompt
+    p_off = 2 * (np.log(2) * (U * (D * sums + 2 * top) + k_off * sums) + 2 * U)
+    tol = mag * (p_off + v_off + (max(max(lens), 1) + 64) * U)
     if dtype == "bf16":
         tol = tol + H * np.abs(out) + H * H / 2 * mag
     assert (np.abs(got - out)[own] <= tol[own] + 1e-37).all()
-    norm = (4 * top + 16) * U + (H if dtype == "bf16" else 0)
+    norm = (4 * top + 16) * U + (H if dtype == "bf16" else 0) + 2 * k_off * root + v_off
     err = np.linalg.norm(got[own] - out[own]) / max(np.linalg.norm(out[own]), 1e-30)
     assert err <= norm or not out[own].any()
     if weights:
         most = np.maximum(np.abs(exp_score), 1.0)
         assert (np.abs(score - exp_score) <= most * (p_off + 300 * U)).all()
-        assert np.linalg.norm(score - exp_score) <= norm_of(top) * np.linalg.norm(exp_score)
+        assert np.linalg.norm(score - exp_score) <= (norm_of(top) + 2 * k_off * root) * np.linalg.norm(exp_score)
     return err
 
 
@@ -585,12 +596,14 @@ def test_prompt_decode_evict_decode(hip, fmt, dtype):
         for r, b, t in kvref.rows_of(qs, held):
             pl = kvref.place(now, tab[b], t)
             score[pl[0], :, pl[1]] = 0
-        out, mag, (top, sums), score = kvref.attention(now, host(st["q"]), qs, held, tab, 128 ** -0.5,
-                                                       0, 1)
-        tol = (4 * top + 16) * U + (H if dtype == "bf16" else 0)
+        out, mag, (top, _, root), score = kvref.attention(now, host(st["q"]), qs, held, tab,
+                                                          128 ** -0.5, 0, 1)
+        f = 2.0 ** -12 if st is p else 0.0
+        k_off = (2 * f if fmt == 4 else 0) if dtype == "bf16" else 6 * U * (st is p)
+        tol = (4 * top + 16) * U + (H if dtype == "bf16" else 0) + 2 * k_off * root + 3 * f
         assert np.linalg.norm(host(st["out"]) - out) <= tol * np.linalg.norm(out)
         assert np.linalg.norm(host(st["arr"]["score"]) - score) <= \
-            (4 * top + 64) * U * np.linalg.norm(score)
+            ((4 * top + 64) * U + 2 * k_off * root) * np.linalg.norm(score)
 
     step(p, [60, 41])
     step(p, [60, 41])
