@@ -758,8 +758,9 @@ AttnPlan kv4_attention_plan(int fmt, int dtype, int head_dim, int n_kv, int n_q,
     const long long rows = (long long)max_new * (n_q / n_kv), pairs = (long long)n_kv * n_seq;
     if (rows > 48)
         p.waves = head_dim <= 128 && (rows + 255) / 256 * pairs >= 192 ? 8 : 4;
+    if (getenv("KVWAVES")) p.waves = atoi(getenv("KVWAVES"));
     const int tile = p.waves ? 32 * p.waves : 16, least = p.waves ? 512 : 128;
-    const int fill = p.waves ? 256 : fmt == 7 && dtype == KV4_BF16 ? 2048 : 768;
+    const int fill = p.waves ? (getenv("KVF") ? atoi(getenv("KVF")) : 256) : fmt == 7 && dtype == KV4_BF16 ? 2048 : 768;
     p.tiles = (int)std::min(32768ll, (rows + tile - 1) / tile);
     const long long want = std::max(1ll, std::min(64ll, fill / (p.tiles * pairs)));
     p.chunk = (int)std::max((long long)least, ((max_len + want - 1) / want + 127) / 128 * 128);

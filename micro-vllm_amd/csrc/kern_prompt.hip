@@ -12,7 +12,8 @@
 // keeps its 11 bits.  bf16 queries and MXFP4 codes times their scales are then exact; int4 codes
 // times their scales, and probabilities, are rounded by 2^-12 of themselves (bf16 outputs round
 // by 2^-8; bf16 operands would have added as much again).  f32 calls take two f16 terms of
-// each rounded operand and leave out the product of the two second ones (2^-23).
+// each rounded operand and leave out the product of the two second ones (2^-23); calls that
+// collect weights two of the keys.
 //
 // A tile's scales are prepared by one wave, in turn, two tiles ahead: it takes the powers out,
 // zeroes the scales of tokens that are not there, and gives a token whose value scales are not
@@ -45,6 +46,19 @@ __device__ __forceinline__ float col_sum(float x) {
     x += __shfl_xor(x, 16);
     return x + __shfl_xor(x, 32);
 }
+// Largest of the wave's values, each not negative (ordered as their bits).
+__device__ __forceinline__ float wave_top(float x) {
+    uint32_t v = __float_as_uint(x);
+#define TOP_STEP(ctrl) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, false))
+    TOP_STEP(0x111);  // row_shr:1, 2, 4, 8, then the rows' last lanes on to the next rows
+    TOP_STEP(0x112);
+    TOP_STEP(0x114);
+    TOP_STEP(0x118);
+    TOP_STEP(0x142);
+    TOP_STEP(0x143);
+#undef TOP_STEP
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)v, 63));
+}
 __device__ __forceinline__ int exponent(float x) { return (int)((__float_as_uint(x) >> 23) & 255u) - 127; }
 
 // What the scale wave says of a tile.
@@ -53,21 +67,26 @@ struct TileInfo {
     uint32_t there[2];       // bit t: token t of the tile exists
 };
 
-template <int FMT, int NG, typename T> struct PromptShape {
+// LSE: the call collects weights, so the rows' sums are held to f32: keys in two terms.
+template <int FMT, int NG, typename T, bool LSE> struct PromptShape {
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int D = 64 * NG, KS = 2 * NG, NF = 4 * NG;  // 32-element steps, row blocks
-    static constexpr int KT = F32 && FMT == 4 && NG >= 3 ? 32 : 64;
-    static constexpr int QT = F32 ? 2 : 1, KVT = F32 && FMT == 4 ? 2 : 1;  // terms
-    static constexpr int SB = FMT == 4 ? NG : 2 * NG;                      // scales of a row
+    static constexpr int KT = (F32 || LSE) && FMT == 4 && NG >= 3 ? 32 : 64;
+    // terms of queries and probabilities, of keys, of values
+    static constexpr int QT = F32 ? 2 : 1;
+    static constexpr int KKT = FMT == 4 && (F32 || LSE) ? 2 : 1, KVT = FMT == 4 && F32 ? 2 : 1;
+    static constexpr int SB = FMT == 4 ? NG : 2 * NG;  // scales of a row
     // a scale as the decoding reads it: f16 where the product is rounded to f16 anyway
-    using Scale = std::conditional_t<FMT == 4 && !F32, _Float16, float>;
+    using KScale = std::conditional_t<FMT == 4 && KKT == 1, _Float16, float>;
+    using VScale = std::conditional_t<FMT == 4 && KVT == 1, _Float16, float>;
     struct Buf {
-        h8 k[KVT][KT / 16][KS][64];
+        h8 k[KKT][KT / 16][KS][64];
         h8 v[KVT][KT / 32][NF][64];
     };
     struct Lds {
         Buf buf[2];
-        Scale sk[2][SB][KT], sv[2][SB][KT];
+        KScale sk[2][SB][KT];
+        VScale sv[2][SB][KT];
         TileInfo info[4];
     };
 };
@@ -75,84 +94,97 @@ template <int FMT, int NG, typename T> struct PromptShape {
 // (n - 8) of the nibbles of one dword's low bits, as f16 pairs: the two nibbles at bits 0 and 16
 // (o[0]) and at bits 4 and 20 (o[1]).  A nibble in the mantissa of 1024 (or, 4 bits up, of 64)
 // adds itself.
-__device__ __forceinline__ void int4_pairs(uint32_t x, h2 &a, h2 &b) {
-    a = as_h2((x & 0x000f000fu) | 0x64006400u) - h2{(_Float16)1032.f, (_Float16)1032.f};
-    b = as_h2((x & 0x00f000f0u) | 0x54005400u) - h2{(_Float16)72.f, (_Float16)72.f};
-}
+struct Int4Pairs {
+    uint32_t m1024 = 0x64006400u, m64 = 0x54005400u;
 
-template <int FMT, int NG, typename T, int W> struct Prompt {
-    using S = PromptShape<FMT, NG, T>;
-    static constexpr int KT = S::KT, KS = S::KS, NF = S::NF, KVT = S::KVT, SB = S::SB, D = S::D;
+    // The constants in vector registers: masking and inserting are one instruction then.
+    __device__ __forceinline__ Int4Pairs() { asm("" : "+v"(m1024), "+v"(m64)); }
+    __device__ __forceinline__ void operator()(uint32_t x, h2 &a, h2 &b) const {
+        a = as_h2((x & 0x000f000fu) | m1024) - h2{(_Float16)1032.f, (_Float16)1032.f};
+        b = as_h2((x & 0x00f000f0u) | m64) - h2{(_Float16)72.f, (_Float16)72.f};
+    }
+};
+
+template <int FMT, int NG, typename T, int W, bool LSE> struct Prompt {
+    using S = PromptShape<FMT, NG, T, LSE>;
+    static constexpr int KT = S::KT, KS = S::KS, NF = S::NF, KKT = S::KKT, KVT = S::KVT;
+    static constexpr int SB = S::SB, D = S::D;
     static constexpr int U = KT * KS;                     // units of keys, and of values
     static constexpr int NT = 64 * W, NU = (2 * U + NT - 1) / NT;  // a thread's units
 
     const AttnArgs &A;
     typename S::Lds &L;
     const int *table;
-    int head, s0, s1, n_tiles;
+    int head, s0, s1, wave;
 
     // One unit of a tile on its way: 32 codes.  Keys: 16 bytes of one token (elements 32 p..);
     // values: elements 64 G + 4 m + j of the 8 tokens of one lane of the second product.
     struct Unit {
-        int phys[2];
-        uint32_t w[4];
+        int entry[2];  // of the table, as loaded
+        uint4 k;
+        uint16_t v[8];
     };
     Unit u[NU];
 
-    __device__ __forceinline__ int phys_of(int t) const {
-        return max(kv4_phys(A.c, table, A.s.max_pages, kv4_page_of(A.c, t)), 0);
+    // A token's table entry: loaded a tile ahead and looked at only where it is used, so that no
+    // wave waits for it.
+    __device__ __forceinline__ int entry_of(int t) const {
+        return table[min(kv4_page_of(A.c, t), A.s.max_pages - 1)];
+    }
+    __device__ __forceinline__ int page_of(int t, int entry) const {  // -1: none
+        return kv4_page_of(A.c, t) < A.s.max_pages && (unsigned)entry < (unsigned)A.c.n_pages ? entry
+                                                                                              : -1;
     }
     __device__ __forceinline__ int slot_of(int t) const { return t - kv4_page_of(A.c, t) * A.c.page; }
 
-    // The pool pages of the units' tokens in a tile (page 0 stands in for none).
+    // The table entries of the units' tokens in a tile.
     __device__ __forceinline__ void look(int tile) {
         const int t0 = s0 + tile * KT;
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
-            const int n = (int)threadIdx.x + i * NT;
-            if (n < U) {
-                u[i].phys[0] = phys_of(t0 + n / (16 * KS) * 16);
-            } else if (n < 2 * U) {
+            const int n = (int)threadIdx.x + i * NT, w = 64 * wave + i * NT;  // (U % 64 = 0)
+            if (w < U) {
+                u[i].entry[0] = entry_of(t0 + n / (16 * KS) * 16);
+            } else if (w < 2 * U) {
                 const int b = (n - U) / (64 * NG);
-                u[i].phys[0] = phys_of(t0 + 32 * b);
-                u[i].phys[1] = phys_of(t0 + 32 * b + 16);
+                u[i].entry[0] = entry_of(t0 + 32 * b);
+                u[i].entry[1] = entry_of(t0 + 32 * b + 16);
             }
         }
     }
+    // Their codes (page 0's in place of none).
     __device__ __forceinline__ void fetch(int tile) {
         const int t0 = s0 + tile * KT;
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
-            const int n = (int)threadIdx.x + i * NT;
-            if (n < U) {
+            const int n = (int)threadIdx.x + i * NT, w = 64 * wave + i * NT;
+            if (w < U) {
                 const int m = n & 15, p = (n >> 4) % KS, t = t0 + n / (16 * KS) * 16;
-                const size_t r = kv4_row(A.c, u[i].phys[0], head, slot_of(t) + m);
-                const uint4 x = *reinterpret_cast<const uint4 *>(A.c.k + r * (D / 2) + 16 * p);
-                u[i].w[0] = x.x; u[i].w[1] = x.y; u[i].w[2] = x.z; u[i].w[3] = x.w;
-            } else if (n < 2 * U) {
+                const size_t r = kv4_row(A.c, max(page_of(t, u[i].entry[0]), 0), head, slot_of(t) + m);
+                u[i].k = *reinterpret_cast<const uint4 *>(A.c.k + r * (D / 2) + 16 * p);
+            } else if (w < 2 * U) {
                 const int v = n - U, m = v & 15, kg = (v >> 4) & 3, G = (v >> 6) % NG;
                 const int t = t0 + v / (64 * NG) * 32;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const size_t r = kv4_row(A.c, u[i].phys[h], head, slot_of(t + 16 * h) + 4 * kg);
+                    const int th = t + 16 * h, pg = max(page_of(th, u[i].entry[h]), 0);
+                    const size_t r = kv4_row(A.c, pg, head, slot_of(th) + 4 * kg);
                     const uint8_t *x = A.c.v + r * (D / 2) + 32 * G + 2 * m;
-                    uint32_t y[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        y[e] = *reinterpret_cast<const uint16_t *>(x + e * (D / 2));
-                    u[i].w[2 * h] = y[0] | (y[1] << 16);
-                    u[i].w[2 * h + 1] = y[2] | (y[3] << 16);
+                        u[i].v[4 * h + e] = *reinterpret_cast<const uint16_t *>(x + e * (D / 2));
                 }
             }
         }
     }
 
     // (n - 8) * s as f16, or as two terms of the f32 product.
-    __device__ __forceinline__ static void scaled(h2 n, float s0, float s1, h2 (&o)[KVT]) {
-        if constexpr (KVT == 2) {
+    template <int N>
+    __device__ __forceinline__ static void scaled(h2 n, float s0, float s1, h2 (&o)[N]) {
+        if constexpr (N == 2) {
             const float a = (float)n[0] * s0, b = (float)n[1] * s1;
             o[0] = round2(a, b);
-            o[KVT - 1] = round2(a - (float)o[0][0], b - (float)o[0][1]);
+            o[N - 1] = round2(a - (float)o[0][0], b - (float)o[0][1]);
         } else {
             o[0] = n * h2{(_Float16)s0, (_Float16)s1};
         }
@@ -161,35 +193,37 @@ template <int FMT, int NG, typename T, int W> struct Prompt {
     // Decodes the fetched tile into its buffer.
     __device__ __forceinline__ void decode(int tile) {
         auto &B = L.buf[tile & 1];
+        const Int4Pairs int4_pairs;
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
-            const int n = (int)threadIdx.x + i * NT;
-            if (n < U) {
+            const int n = (int)threadIdx.x + i * NT, w = 64 * wave + i * NT;
+            if (w < U) {
+                const uint32_t word[4] = {u[i].k.x, u[i].k.y, u[i].k.z, u[i].k.w};
                 const int m = n & 15, p = (n >> 4) % KS, st = n / (16 * KS);
                 const auto s = L.sk[tile & 1][FMT == 4 ? p / 2 : p][st * 16 + m];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    h8 o[KVT];
+                    h8 o[KKT];
                     if constexpr (FMT == 4) {  // order 0 4 1 5 2 6 3 7
                         h2 x[4];
-                        int4_pairs(u[i].w[j], x[0], x[1]);
-                        int4_pairs(u[i].w[j] >> 8, x[2], x[3]);
+                        int4_pairs(word[j], x[0], x[1]);
+                        int4_pairs(word[j] >> 8, x[2], x[3]);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            h2 y[KVT];
+                            h2 y[KKT];
                             scaled(x[e], (float)s, (float)s, y);
 #pragma unroll
-                            for (int k = 0; k < KVT; ++k) {
+                            for (int k = 0; k < KKT; ++k) {
                                 o[k][2 * e] = y[k][0];
                                 o[k][2 * e + 1] = y[k][1];
                             }
                         }
                     } else {
                         const h2 x[4] = {
-                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(u[i].w[j], (float)s, 0),
-                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(u[i].w[j], (float)s, 1),
-                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(u[i].w[j], (float)s, 2),
-                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(u[i].w[j], (float)s, 3)};
+                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word[j], (float)s, 0),
+                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word[j], (float)s, 1),
+                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word[j], (float)s, 2),
+                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word[j], (float)s, 3)};
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             o[0][2 * e] = x[e][0];
@@ -197,10 +231,10 @@ template <int FMT, int NG, typename T, int W> struct Prompt {
                         }
                     }
 #pragma unroll
-                    for (int k = 0; k < KVT; ++k)
+                    for (int k = 0; k < KKT; ++k)
                         B.k[k][st][p][j * 16 + m] = o[k];
                 }
-            } else if (n < 2 * U) {
+            } else if (w < 2 * U) {
                 const int v = n - U, m = v & 15, kg = (v >> 4) & 3, G = (v >> 6) % NG;
                 const int b = v / (64 * NG);
                 const auto *sp = L.sv[tile & 1][FMT == 4 ? G : 2 * G + (m >> 3)] + 32 * b + 4 * kg;
@@ -209,7 +243,7 @@ template <int FMT, int NG, typename T, int W> struct Prompt {
                 for (int e = 0; e < 4; ++e) {  // tokens 2 e and 2 e + 1 of the lane's eight
                     const auto s0 = sp[16 * (e >> 1) + 2 * (e & 1)];
                     const auto s1 = sp[16 * (e >> 1) + 2 * (e & 1) + 1];
-                    const uint32_t x = u[i].w[e];
+                    const uint32_t x = u[i].v[2 * e] | ((uint32_t)u[i].v[2 * e + 1] << 16);
                     h2 y[4][KVT];
                     if constexpr (FMT == 4) {
                         h2 z[4];
@@ -248,11 +282,15 @@ template <int FMT, int NG, typename T, int W> struct Prompt {
 
     // ---- the scale wave: lane t is token t of the tile (KT = 32: the upper half repeats it)
     float sk[FMT == 4 ? NG : 2 * NG], sv[FMT == 4 ? NG : 2 * NG];
+    int entry;
     bool there;
 
+    __device__ __forceinline__ void look_scales(int tile) {
+        entry = entry_of(s0 + tile * KT + ((int)threadIdx.x & (KT - 1)));
+    }
     __device__ __forceinline__ void fetch_scales(int tile) {
         const int t = s0 + tile * KT + ((int)threadIdx.x & (KT - 1));
-        const int phys = t < s1 ? kv4_phys(A.c, table, A.s.max_pages, kv4_page_of(A.c, t)) : -1;
+        const int phys = t < s1 ? page_of(t, entry) : -1;
         there = phys >= 0;
         const size_t r = there ? kv4_row(A.c, phys, head, slot_of(t)) : 0;
 #pragma unroll
@@ -280,11 +318,8 @@ template <int FMT, int NG, typename T, int W> struct Prompt {
             mk = fmaxf(mk, nonfinite(sk[g]) ? 0.f : fabsf(sk[g]));
             mv = fmaxf(mv, fabsf(sv[g]));
         }
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) {
-            mk = fmaxf(mk, __shfl_xor(mk, o));
-            mv = fmaxf(mv, __shfl_xor(mv, o));
-        }
+        mk = wave_top(mk);
+        mv = wave_top(mv);
         const int ek = mk > 0.f ? exponent(mk) - TOP : 0;
         int ev = tile > 0 ? L.info[(tile - 1) & 3].ev : -1000;
         ev = mv > 0.f ? max(ev, exponent(mv) - TOP) : ev;
@@ -293,8 +328,8 @@ template <int FMT, int NG, typename T, int W> struct Prompt {
 #pragma unroll
             for (int g = 0; g < SB; ++g) {
                 const float k = there && !good ? NAN : ldexpf(sk[g], -ek);
-                L.sk[tile & 1][g][t] = (typename S::Scale)k;
-                L.sv[tile & 1][g][t] = (typename S::Scale)ldexpf(sv[g], -max(ev, -400));
+                L.sk[tile & 1][g][t] = (typename S::KScale)k;
+                L.sv[tile & 1][g][t] = (typename S::VScale)ldexpf(sv[g], -max(ev, -400));
             }
         }
         if (lane == 0) {
@@ -309,10 +344,14 @@ template <int FMT, int NG, typename T, int W> struct Prompt {
 
 }  // namespace
 
-template <int FMT, int NG, typename T, int W>
-__global__ __launch_bounds__(64 * W, W / 4) void k_kv4_prompt(AttnArgs A) {
-    using S = PromptShape<FMT, NG, T>;
-    constexpr int D = S::D, KT = S::KT, KS = S::KS, NF = S::NF, QT = S::QT, KVT = S::KVT;
+template <int FMT, int NG, typename T, int W, bool LSE>
+__global__ __launch_bounds__(64 * W, NG <= 2 ? 2 : 1) void k_kv4_prompt(AttnArgs A) {
+    using S = PromptShape<FMT, NG, T, LSE>;
+    constexpr int D = S::D, KT = S::KT, KS = S::KS, NF = S::NF, QT = S::QT;
+    constexpr int KKT = S::KKT, KVT = S::KVT;
+    // The rows' sums come with the values' products, of the probabilities as rounded; where they
+    // have to be f32 and one term is all there is, from the f32 ones.
+    constexpr bool SUMS = LSE && QT == 1;
     // Probabilities are carried as 2^(x - ref): up to 2^15 in f16, and so that a maximum that is
     // not raised yet (it may pass by 2^SLACK) still fits.
     constexpr float SLACK = S::F32 ? 1.f : 8.f, LIFT = 15.f - SLACK;
@@ -332,7 +371,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_kv4_prompt(AttnArgs A) {
         const int s0 = max(lo & ~(KT - 1), split * A.chunk);
         const int s1 = split + 1 == A.splits ? hi : min(hi, (split + 1) * A.chunk);
         const int n_tiles = s1 > s0 ? (s1 - s0 + KT - 1) / KT : 0;
-        Prompt<FMT, NG, T, W> P{A, L, A.s.table + (size_t)seq * A.s.max_pages, head, s0, s1, n_tiles};
+        Prompt<FMT, NG, T, W, LSE> P{A, L, A.s.table + (size_t)seq * A.s.max_pages, head, s0, s1, wave};
 
         // the wave's rows: columns col and 16 + col
         const int w0 = base + 32 * wave, w1 = min(rows, w0 + 32);
@@ -384,13 +423,22 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_kv4_prompt(AttnArgs A) {
 #pragma unroll
         for (int f = 0; f < NF; ++f)
             o[f][0] = o[f][1] = f4v{0.f, 0.f, 0.f, 0.f};
-        float ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // ref: see LIFT
+        // the rows' sums of probabilities (in every row of the accumulator); ref: see LIFT
+        f4v l[2] = {f4v{0.f, 0.f, 0.f, 0.f}, f4v{0.f, 0.f, 0.f, 0.f}};
+        float ref[2] = {-INFINITY, -INFINITY};
+        h8 ones;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            ones[i] = (_Float16)1.f;
         int ev = -1000;
 
         if (n_tiles > 0) {
             P.look(0);
-            if (wave < 2) {
-                P.fetch_scales(wave);  // a tile behind the last: nothing there
+            // (a tile behind the last: nothing there)
+            P.look_scales(wave);
+            if (wave < 3) {
+                P.fetch_scales(wave);
+                P.look_scales(wave + W);
             }
             P.fetch(0);
             P.look(1);
@@ -400,17 +448,20 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_kv4_prompt(AttnArgs A) {
             if (wave == 1)
                 P.put_scales(1);
             P.decode(0);
+            P.fetch(1);
+            P.look(2);
             __syncthreads();
         }
         for (int tile = 0; tile < n_tiles; ++tile) {
-            const bool more = tile + 1 < n_tiles;
-            const bool scales = tile + 2 < n_tiles && wave == (tile + 2) % W;
-            if (scales)
-                P.fetch_scales(tile + 2);
-            if (more) {
-                P.fetch(tile + 1);
-                P.look(tile + 2);
+            if (wave == (tile + 2) % W)
+                P.put_scales(tile + 2);
+            if (wave == (tile + 3) % W) {
+                P.fetch_scales(tile + 3);
+                P.look_scales(tile + 3 + W);
             }
+            P.decode(tile + 1);  // (of a tile behind the last: zeros)
+            P.fetch(tile + 2);
+            P.look(tile + 3);
             const int t0 = s0 + tile * KT;
             const TileInfo I = L.info[tile & 3];
             const auto &B = L.buf[tile & 1];
@@ -422,10 +473,12 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_kv4_prompt(AttnArgs A) {
 #pragma unroll
                     for (int p = 0; p < KS; ++p) {
 #pragma unroll
-                        for (int k = KVT - 1; k >= 0; --k) {
+                        for (int k = KKT - 1; k >= 0; --k) {
                             const h8 a = B.k[k][b][p][lane];
 #pragma unroll
-                            for (int t = QT - 1 - k; t >= 0; --t) {
+                            for (int t = (KKT > QT ? KKT : QT) - 1 - k; t >= 0; --t) {
+                                if (t >= QT)
+                                    continue;
                                 s[b][0] = mfma16(a, q[0][p][t], s[b][0]);
                                 s[b][1] = mfma16(a, q[1][p][t], s[b][1]);
                             }
@@ -466,9 +519,10 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_kv4_prompt(AttnArgs A) {
                     const float k2lo = S::F32 ? ldexpf(fabsf(A.scale2) == A.scale2 ? A.scale2_lo : -A.scale2_lo, I.ek + eq[c]) : 0.f;
                     float top = -INFINITY;
 #pragma unroll
-                    for (int b = 0; b < KT / 16; ++b)
-                        top = fmaxf(top, fmaxf(fmaxf(s[b][c][0], s[b][c][1]),
-                                               fmaxf(s[b][c][2], s[b][c][3])));
+                    for (int b = 0; b < KT / 16; ++b) {
+                        top = fmaxf(fmaxf(top, s[b][c][0]), s[b][c][1]);
+                        top = fmaxf(fmaxf(top, s[b][c][2]), s[b][c][3]);
+                    }
                     top = top * k2 - LIFT;
                     if (__any(top > ref[c] + SLACK)) {
                         const float up = fmaxf(ref[c], col_max(top));
@@ -493,7 +547,9 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_kv4_prompt(AttnArgs A) {
                             else
                                 p[i] = __builtin_amdgcn_exp2f(fmaf(x, k2, -r));
                         }
-                        l[c] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                        if constexpr (SUMS)
+                            l[c][0] += ((p[0] + p[1]) + (p[2] + p[3])) +
+                                       ((p[4] + p[5]) + (p[6] + p[7]));
 #pragma unroll
                         for (int k = 0; k < QT; ++k)
 #pragma unroll
@@ -507,7 +563,12 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_kv4_prompt(AttnArgs A) {
                     }
                 }
 #pragma unroll
-                for (int b = 0; b < KT / 32; ++b)
+                for (int b = 0; b < KT / 32; ++b) {
+#pragma unroll
+                    for (int t = SUMS ? -1 : QT - 1; t >= 0; --t) {
+                        l[0] = mfma16(ones, pr[0][b][t], l[0]);
+                        l[1] = mfma16(ones, pr[1][b][t], l[1]);
+                    }
 #pragma unroll
                     for (int n = 0; n < NF; ++n)
 #pragma unroll
@@ -519,16 +580,13 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_kv4_prompt(AttnArgs A) {
                                 o[n][1] = mfma16(a, pr[1][b][t], o[n][1]);
                             }
                         }
+                }
             }
-            if (more)
-                P.decode(tile + 1);
-            if (scales)
-                P.put_scales(tile + 2);
             __syncthreads();
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const float sum = col_sum(l[c]);
+            const float sum = SUMS ? col_sum(l[c][0]) : l[c][0];
             if (live[c]) {
                 const int tok = q0 + row[c] / A.group, hq = head * A.group + row[c] % A.group;
                 const size_t at = ((size_t)split * A.s.n_tok + tok) * A.n_q + hq;
@@ -568,18 +626,26 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_kv4_prompt(AttnArgs A) {
     }
 }
 
-template <int FMT, int NG, typename T, int W>
-static hipError_t prompt(const AttnArgs &a, hipStream_t st) {
-    using Lds = typename PromptShape<FMT, NG, T>::Lds;
+template <int FMT, int NG, typename T, int W, bool LSE>
+static hipError_t prompt_one(const AttnArgs &a, hipStream_t st) {
+    using Lds = typename PromptShape<FMT, NG, T, LSE>::Lds;
     static_assert(sizeof(Lds) <= 160 * 1024, "LDS");
     static const hipError_t lds = hipFuncSetAttribute(
-        reinterpret_cast<const void *>(&k_kv4_prompt<FMT, NG, T, W>),
+        reinterpret_cast<const void *>(&k_kv4_prompt<FMT, NG, T, W, LSE>),
         hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Lds));
     if (lds != hipSuccess)
         return lds;
     const dim3 grid((unsigned)a.c.n_kv, (unsigned)a.s.n_seq, (unsigned)(a.splits * a.tiles));
-    hipLaunchKernelGGL((k_kv4_prompt<FMT, NG, T, W>), grid, dim3(64 * W), sizeof(Lds), st, a);
+    hipLaunchKernelGGL((k_kv4_prompt<FMT, NG, T, W, LSE>), grid, dim3(64 * W), sizeof(Lds), st, a);
     return hipGetLastError();
+}
+
+template <int FMT, int NG, typename T, int W>
+static hipError_t prompt(const AttnArgs &a, hipStream_t st) {
+    if constexpr (sizeof(T) == 2)  // (f32 calls hold their sums to f32 anyway)
+        return a.lse ? prompt_one<FMT, NG, T, W, true>(a, st)
+                     : prompt_one<FMT, NG, T, W, false>(a, st);
+    return prompt_one<FMT, NG, T, W, false>(a, st);
 }
 
 template <int FMT, typename T>

@@ -14,8 +14,8 @@ inline uint32_t kv4_page_rcp(int page) {
     return p == 1 ? 0u : (uint32_t)((uint64_t(1) << 32) / p) + 1u;
 }
 __device__ __forceinline__ int kv4_page_of(const Kv4View &c, int t) {
-    const uint32_t u = (uint32_t)t >> 4;
-    return (int)(c.rcp ? __umulhi(u, c.rcp) : u);
+    const uint32_t u = (uint32_t)t >> 4, q = __umulhi(u, c.rcp);
+    return (int)(c.rcp ? q : u);
 }
 
 // The pool page of a sequence's page pg, or -1 where there is none.

@@ -15,7 +15,8 @@ Bars, by the roundings that can meet (u = 2^-24, half an f32 step; h = 2^-8, hal
   keys (an exponent is off by 2 f of sum |q k|) and of values (2 f of sum P |v|); MXFP4 is exact.
   f32 calls hold each rounded operand in two terms (f^2 of it, 2^-24, taken as 2 u for its
   subnormal second terms) and leave out the product of the second two (f^2): 3 * 2 u of sum
-  |q k| and of sum P |v|.
+  |q k| and of sum P |v|.  So do the exponents of calls that collect weights, whose own sums
+  take exact products.
 - the 2-norm: errors of independent roundings grow as their root: exponents 4 u of the largest
   one, 16 u beside; f16 keys' 2 f of the root of the sum of (q k)^2, twice for the
   denominator's share; f16 values and probabilities 3 f.
@@ -237,6 +238,9 @@ def check_attention(c, q, got, score, q_start, lens, tab, scale, window, weights
     f = 2.0 ** -12 if prompt else 0.0
     k_off = (2 * f if c["fmt"] == 4 else 0) if dtype == "bf16" else 6 * U * prompt
     v_off = (3 * f if c["fmt"] == 4 else f) if dtype == "bf16" else 6 * U * prompt
+    w_off = 6 * U * prompt
+    if weights:
+        k_off = w_off
     p_off = 2 * (np.log(2) * (U * (D * sums + 2 * top) + k_off * sums) + 2 * U)
     tol = mag * (p_off + v_off + (max(max(lens), 1) + 64) * U)
     if dtype == "bf16":
@@ -598,8 +602,7 @@ def test_prompt_decode_evict_decode(hip, fmt, dtype):
             score[pl[0], :, pl[1]] = 0
         out, mag, (top, _, root), score = kvref.attention(now, host(st["q"]), qs, held, tab,
                                                           128 ** -0.5, 0, 1)
-        f = 2.0 ** -12 if st is p else 0.0
-        k_off = (2 * f if fmt == 4 else 0) if dtype == "bf16" else 6 * U * (st is p)
+        f, k_off = (2.0 ** -12, 6 * U) if st is p else (0.0, 0.0)
         tol = (4 * top + 16) * U + (H if dtype == "bf16" else 0) + 2 * k_off * root + 3 * f
         assert np.linalg.norm(host(st["out"]) - out) <= tol * np.linalg.norm(out)
         assert np.linalg.norm(host(st["arr"]["score"]) - score) <= \
