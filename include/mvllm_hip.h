@@ -137,6 +137,8 @@ int mvllm_hip_moe_block_dev_noalloc(int nb, int D, int Iinter, int fmt, int qgs,
  *   "dec_inline" 1 (default) = the decode gate/up launch carries its descriptors in
  *            its kernel arguments (at most 64 items; same results); 0 = it reads them
  *            from the pinned plan slot.
+ *   "kv4_rows" mvllm_hip_kv4_attention_dev: 0 = automatic, 1 = the 16-row kernel, 2 = the kernel
+ *            of many rows, at every size.
  *   "dequant_path" 1 = mvllm_hip_dequant decodes through the matrix-core operand path.
  * fmt 0 experts (f32 weights, the shared experts) run on the f32 matrix cores when
  * D % 16 == 0, Iinter % 32 == 0, D % 32 == 0 and rows are 16-byte aligned.  Shapes the
@@ -349,9 +351,13 @@ int mvllm_hip_kv4_read_dev(const mvllm_kv4 *cache, int dtype, void *k, void *v, 
  * query head h of the new token at position p (its index among the sequence's lens[b] tokens)
  * = sum_j P_j v_j over the tokens j <= p (and j > p - window where window > 0) of kv head h /
  * (n_q / n_kv), P = softmax(scale * q . k_j).  A row that sees no token gives zeros.
- * Products: the codes enter the bf16 matrix cores exactly; f32 queries and probabilities as
- * three bf16 terms (all 24 bits), bf16 queries exactly and their probabilities as two terms;
- * sums, maxima and exponentials are f32.
+ * Up to 16 rows (new tokens x heads of the group) of a sequence and kv head, and calls of more
+ * that are short: the codes enter the bf16 matrix cores exactly; f32 queries and probabilities
+ * as three bf16 terms (all 24 bits), bf16 queries exactly and their probabilities as two terms.
+ * Long calls of more rows run on f16 operands with powers of two taken out: bf16 calls round
+ * probabilities, and int4 codes times their scales, once by 2^-12; f32 calls hold such operands in
+ * two terms (2^-23), and so do the exponents of calls that collect weights.  Sums, maxima and
+ * exponentials are f32.
  * weights: 1 adds to score, 2 stores into it, for each of the sequences' tokens, the sum of its
  * P over the call's new tokens and the kv head's group of query heads (0 where none sees it).
  * Sequences that share pages may attend together with weights 0; their scores would be two

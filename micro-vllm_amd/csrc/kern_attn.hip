@@ -19,6 +19,18 @@ __device__ __forceinline__ f4v mfma(bf16x8 a, bf16x8 b, f4v c) {
 __device__ __forceinline__ bf16x2 as_bf2(uint32_t u) { return __builtin_bit_cast(bf16x2, u); }
 __device__ __forceinline__ uint32_t as_u32(bf16x2 b) { return __builtin_bit_cast(uint32_t, b); }
 
+// Sum over the 16 lanes of a row, in each of them.
+__device__ __forceinline__ float row_sum(float x) {
+#define ROW_STEP(ctrl)                                                                         \
+    x += __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), ctrl, \
+                                                               0xf, 0xf, false))
+    ROW_STEP(0x128);  // row_ror:8, 4, 2, 1
+    ROW_STEP(0x124);
+    ROW_STEP(0x122);
+    ROW_STEP(0x121);
+#undef ROW_STEP
+    return x;
+}
 // Maximum and sum over the four lanes that hold one matrix column (lane, +16, +32, +48).
 __device__ __forceinline__ float col_max(float x) {
     x = fmaxf(x, __shfl_xor(x, 16));
@@ -464,8 +476,8 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
         const int r1 = min(t.rows, r0 + 16);
         int lo, hi;
         span_of(A, t, r0, r1, lo, hi);
-        const int s0 = max(lo & ~31, split * A.chunk);
-        const int s1 = split + 1 == A.splits ? hi : min(hi, (split + 1) * A.chunk);
+        const int s0 = (lo & ~31) + split * A.chunk;
+        const int s1 = split + 1 == A.splits ? hi : min(hi, s0 + A.chunk);
         const int row = r0 + col;
         const bool live = row < r1;
         const int pos = t.pos0 + (live ? row : r0) / A.group;
@@ -671,50 +683,78 @@ __global__ __launch_bounds__(256) void k_kv4_join(AttnArgs A) {
         A.lse[at] = L > 0.f ? M + log2f(L) : -INFINITY;
 }
 
-// One wave: the weights of 32 tokens of one sequence and kv head, over all of its rows: the
-// keys stay in registers as operands, the rows pass by 16 at a time, and each token's sum is
-// formed by this wave alone.
-template <int FMT, int NG, typename T>
+// The weights of blocks of 16 NB tokens of one sequence and kv head, over all of its rows.  The
+// keys stay in registers as operands while the rows pass by, 16 at a time, and each token's sum
+// is formed in one place, in one order.
+//
+// FEW (decode): each wave takes blocks of its own, the next one's keys on their way, with the
+// operands of up to 16 rows loaded once.  Otherwise the four waves share a block and take every
+// fourth 16 of its rows: what takes time is the way to the rows, not the products.
+template <int FMT, int NG, typename T, bool FEW>
 __global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs A) {
-    constexpr int TQ = sizeof(T) == 4 ? 3 : 1;
+    constexpr int TQ = sizeof(T) == 4 ? 3 : 1, NB = FEW ? 2 : 4, BLK = 16 * NB;
+    __shared__ float part[FEW ? 1 : 4][BLK];
     const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const Tile t = tile_of(A, blockIdx.z, blockIdx.y);
+    const Tile t = tile_of(A, blockIdx.y, blockIdx.x);
     const int len = kv4_len(A.c, t.len, A.s.max_pages);
-    for (int t0 = (blockIdx.x * 4 + wave) * 32; t0 < len; t0 += gridDim.x * 128) {
-        Keys<FMT, NG> k[2];
-        bool ok[2];
-        size_t at[2];
+    int row = -1, pos = -1, from = -1;
+    float lse = -INFINITY, k8[NG];
+    bool live = false;
+    bf16x8 q[NG][2][TQ];
+    auto rows_at = [&](int r) {
+        row = r + col;
+        live = row < t.rows;
+        pos = t.pos0 + (live ? row : 0) / A.group;
+        from = A.window > 0 ? pos - A.window : -1;
+        lse = live ? A.lse[(size_t)(t.first + row / A.group) * A.n_q + t.head * A.group +
+                           row % A.group]
+                   : -INFINITY;
+        load_q<FMT, NG, TQ, T>(A, t, row, live, q, k8);
+    };
+    Keys<FMT, NG> k[NB], ahead[FEW ? NB : 1];
+    bool ok[NB];
+    size_t at[NB];
+    auto fetch = [&](int t0, Keys<FMT, NG> *to) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int tt = t0 + 16 * h, pg = kv4_page_of(A.c, tt);
-            const int phys = __builtin_amdgcn_readfirstlane(
-                kv4_phys(A.c, t.table, A.s.max_pages, pg));
-            ok[h] = phys >= 0;
-            at[h] = kv4_row(A.c, max(phys, 0), t.head, tt - pg * A.c.page);
-            k[h].load(A.c, at[h]);
+        for (int h = 0; h < NB; ++h) {
+            const Place pl = place_of(A, t, t0 + 16 * h);
+            ok[h] = pl.phys >= 0;
+            at[h] = kv4_row(A.c, max(pl.phys, 0), t.head, pl.slot);
+            to[h].load(A.c, at[h]);
         }
-        float w[2][4] = {};
-        // the first row that may see the first token, and the rows whose window it has left
-        int r = (int)min((long long)t.rows, max(0ll, (long long)t0 - t.pos0) * A.group);
-        int rend = t.rows;
-        if (A.window > 0)
-            rend = min((long long)rend,
-                       max(0ll, (long long)t0 + 31 + A.window - t.pos0) * A.group);
-        for (r &= ~15; r < rend; r += 16) {
-            const int row = r + col;
-            const bool live = row < t.rows;
-            const int pos = t.pos0 + (live ? row : 0) / A.group;
-            const int from = A.window > 0 ? pos - A.window : -1;
-            const float lse =
-                live ? A.lse[(size_t)(t.first + row / A.group) * A.n_q + t.head * A.group +
-                             row % A.group]
-                     : -INFINITY;
-            bf16x8 q[NG][2][TQ];
-            float k8[NG];
-            load_q<FMT, NG, TQ, T>(A, t, row, live, q, k8);
+    };
+    const int step = (int)gridDim.z * (FEW ? 4 : 1) * BLK;
+    int t0 = ((int)blockIdx.z * (FEW ? 4 : 1) + (FEW ? wave : 0)) * BLK;
+    if (FEW && t0 < len)
+        fetch(t0, ahead);
+    const bool once = FEW && t.rows <= 16;
+    if (once && t0 < len)
+        rows_at(0);
+    for (; t0 < len; t0 += step) {
+        bool there[NB];
+        size_t place[NB];
+        if constexpr (FEW) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < NB; ++h) {
+                k[h] = ahead[h];
+                there[h] = ok[h];
+                place[h] = at[h];
+            }
+            if (t0 + step < len)
+                fetch(t0 + step, ahead);
+        } else {
+            fetch(t0, k);
+#pragma unroll
+            for (int h = 0; h < NB; ++h) {
+                there[h] = ok[h];
+                place[h] = at[h];
+            }
+        }
+        float w[NB][4] = {};
+        auto add = [&] {
+#pragma unroll
+            for (int h = 0; h < NB; ++h) {
                 const f4v s = dot_keys<FMT, NG, TQ>(k[h], q, k8);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -723,28 +763,60 @@ __global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs A) {
                     w[h][i] += sees ? power<T>(A, s[i], lse) : 0.f;
                 }
             }
+        };
+        if (once) {
+            add();
+        } else {
+            // from the first row that may see the first token to the last whose window holds
+            // the last one
+            int r = (int)min((long long)t.rows, max(0ll, (long long)t0 - t.pos0) * A.group);
+            int rend = t.rows;
+            if (A.window > 0)
+                rend = (int)min((long long)rend,
+                                max(0ll, (long long)t0 + BLK - 1 + A.window - t.pos0) * A.group);
+            for (r = (r & ~15) + (FEW ? 0 : 16 * wave); r < rend; r += FEW ? 16 : 64) {
+                rows_at(r);
+                add();
+            }
         }
+        // a lane's four tokens of each 16, over the 16 rows of its columns; lane (kg, col < 4)
+        // is left with token 4 kg + col
+        float mine[NB];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < NB; ++h) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
+                w[h][i] = row_sum(w[h][i]);
+            mine[h] = col == 0 ? w[h][0] : col == 1 ? w[h][1] : col == 2 ? w[h][2] : w[h][3];
+        }
+        if constexpr (!FEW) {
+            __syncthreads();  // the block before has been read
+            if (col < 4) {
 #pragma unroll
-                for (int o = 8; o >= 1; o >>= 1)
-                    w[h][i] += __shfl_xor(w[h][i], o);
-            if (col < 4 && ok[h]) {
-                const int tok = t0 + 16 * h + 4 * kg + col;
-                const float x = col == 0 ? w[h][0] : col == 1 ? w[h][1] : col == 2 ? w[h][2]
-                                                                                     : w[h][3];
-                float *p = A.c.score + at[h] + 4 * kg + col;
-                if (tok < len)
-                    *p = A.weights == KV4_WEIGHTS_ADD ? *p + x : x;
+                for (int h = 0; h < NB; ++h)
+                    part[wave][16 * h + 4 * kg + col] = mine[h];
+            }
+            __syncthreads();
+            if (wave > 0)
+                continue;
+#pragma unroll
+            for (int h = 0; h < NB; ++h) {
+                const int n = 16 * h + 4 * kg + (col & 3);
+                mine[h] = (part[0][n] + part[1][n]) + (part[2][n] + part[3][n]);
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < NB; ++h) {
+            if (col < 4 && there[h] && t0 + 16 * h + 4 * kg + col < len) {
+                float *p = A.c.score + place[h] + 4 * kg + col;
+                *p = A.weights == KV4_WEIGHTS_ADD ? *p + mine[h] : mine[h];
             }
         }
     }
 }
 
-// How a call is cut.  Up to 48 rows a sequence and kv head take the 16-row kernel, more the
-// kernel of kern_prompt.hip, with 8 waves (256 rows) a workgroup where that fills the chip.
+// How a call is cut, for the 16-row kernel or (prompt) that of kern_prompt.hip, 8 waves of 32 rows
+// a workgroup (4 for head_dim 192 and 256, whose sums fill the registers).
 //
 // Splits of the tokens: enough workgroups to fill the chip (`fill`), but chunks of 128 tokens
 // (one block a wave) at least, and at most the 64 splits that a wave joins.  A workgroup's
@@ -752,42 +824,67 @@ __global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs A) {
 // CU anyway, three times the CUs are best (768: 16 f32 int4 streams to 4096 tokens 54 us, 58 with
 // 2048, 62 with 512); bf16 over MXFP4, three a CU and less work a block, gains by finer chunks
 // (32 streams to 16384 tokens 110 us with 2048, 120 with 768).
-AttnPlan kv4_attention_plan(int fmt, int dtype, int head_dim, int n_kv, int n_q, int n_tok,
-                            int n_seq, int max_new, int max_len, bool weights) {
+static AttnPlan plan_for(bool prompt, int fmt, int dtype, int head_dim, int n_kv, int n_q,
+                         int n_tok, int n_seq, int max_new, int max_len, int window,
+                         bool weights) {
     AttnPlan p{};
     const long long rows = (long long)max_new * (n_q / n_kv), pairs = (long long)n_kv * n_seq;
-    if (rows > 48)
-        p.waves = head_dim <= 128 && (rows + 255) / 256 * pairs >= 192 ? 8 : 4;
-    if (getenv("KVWAVES")) p.waves = atoi(getenv("KVWAVES"));
-    const int tile = p.waves ? 32 * p.waves : 16, least = p.waves ? 512 : 128;
-    const int fill = p.waves ? (getenv("KVF") ? atoi(getenv("KVF")) : 256) : fmt == 7 && dtype == KV4_BF16 ? 2048 : 768;
+    p.waves = !prompt ? 0 : head_dim <= 128 ? 8 : 4;
+    const int tile = p.waves ? 32 * p.waves : 16, least = p.waves ? 256 : 128;
+    const int fill = p.waves ? 256 : fmt == 7 && dtype == KV4_BF16 ? 2048 : 768;
     p.tiles = (int)std::min(32768ll, (rows + tile - 1) / tile);
+    // the most tokens that a tile's rows see, from a multiple of 64 on
+    const long long seen =
+        window > 0 ? std::min((long long)max_len, (long long)window + tile / (n_q / n_kv) + 65)
+                   : max_len;
     const long long want = std::max(1ll, std::min(64ll, fill / (p.tiles * pairs)));
-    p.chunk = (int)std::max((long long)least, ((max_len + want - 1) / want + 127) / 128 * 128);
-    p.splits = (max_len + p.chunk - 1) / p.chunk;
+    p.chunk = (int)std::max((long long)least, ((seen + want - 1) / want + 127) / 128 * 128);
+    p.splits = (int)((seen + p.chunk - 1) / p.chunk);
     auto add = [&](size_t bytes) {
         const size_t at = p.bytes;
         p.bytes += (bytes + 255) / 256 * 256;
         return at;
     };
+    // room for the splits that any window would have
     const size_t heads = (size_t)n_tok * n_q;
-    if (p.splits > 1) {
-        p.part = add(p.splits * heads * head_dim * 4);
-        p.ml = add(p.splits * heads * 8);
+    const size_t most = (size_t)std::min(want, ((long long)max_len + least - 1) / least);
+    if (most > 1) {
+        p.part = add(most * heads * head_dim * 4);
+        p.ml = add(most * heads * 8);
     }
     if (weights)
         p.lse = add(heads * 4);
     return p;
 }
 
+// More than 16 rows a sequence and kv head take either kernel.  The 16-row one starts sooner and
+// spreads wider; the other reads and decodes a tile of tokens once for 256 rows.  They meet at
+// about 12 million (row, token) pairs of 128 elements, summed over sequences and kv heads, in
+// bf16 (int4, 8 heads, groups of 4: 64 rows of 4 sequences over 4096 tokens 37 and 32 us, 256
+// rows of one 41 and 41, of 8 with a window of 1024 44 and 42, 2048 rows of 4 516 and 173; 128
+// rows of the 8 25 and 34), and at 20 million in f32, whose second terms cost the tiles more.
+AttnPlan kv4_attention_plan(int choice, int fmt, int dtype, int head_dim, int n_kv, int n_q,
+                            int n_tok, int n_seq, int max_new, int max_len, int window,
+                            bool weights) {
+    const double rows = (double)max_new * (n_q / n_kv) * n_kv * n_seq;
+    const double seen = window > 0 ? std::min((double)max_len, (double)window + max_new) : max_len;
+    const bool many = max_new * (long long)(n_q / n_kv) > 16;
+    const bool prompt = choice == 2 || (choice == 0 && many &&
+                                        rows * seen * head_dim >=
+                                            128e6 * (dtype == KV4_BF16 ? 12 : 20));
+    return plan_for(prompt, fmt, dtype, head_dim, n_kv, n_q, n_tok, n_seq, max_new, max_len, window,
+                    weights);
+}
+
 size_t kv4_attention_bytes(int head_dim, int n_kv, int n_q, int n_tok, int n_seq, int max_new,
                            int max_len, bool weights) {
     size_t most = 0;
-    for (int fmt : {4, 7})
-        for (int dtype : {KV4_F32, KV4_BF16})
-            most = std::max(most, kv4_attention_plan(fmt, dtype, head_dim, n_kv, n_q, n_tok, n_seq,
-                                                     max_new, max_len, weights)
-                                      .bytes);
+    for (bool prompt : {false, true})
+        for (int fmt : {4, 7})
+            for (int dtype : {KV4_F32, KV4_BF16})
+                most = std::max(most, plan_for(prompt, fmt, dtype, head_dim, n_kv, n_q, n_tok,
+                                               n_seq, max_new, max_len, 0, weights)
+                                          .bytes);
     return most;
 }
 
@@ -795,8 +892,8 @@ template <int FMT, int NG, typename T>
 static hipError_t attention(const AttnArgs &a, int max_len, hipStream_t st) {
     hipError_t e;
     if (a.waves) {
-        if ((e = launch_kv4_prompt(FMT, 64 * NG, sizeof(T) == 2 ? KV4_BF16 : KV4_F32, a.waves, a,
-                                   st)) != hipSuccess)
+        if ((e = launch_kv4_prompt(FMT, 64 * NG, sizeof(T) == 2 ? KV4_BF16 : KV4_F32, a, st)) !=
+            hipSuccess)
             return e;
     } else {
     // Heads go round the XCDs first, splits last: sequences of unlike length leave the later
@@ -814,10 +911,15 @@ static hipError_t attention(const AttnArgs &a, int max_len, hipStream_t st) {
             return e;
     }
     if (a.weights != KV4_WEIGHTS_NONE) {
-        const unsigned wgs = (unsigned)std::max(1, (max_len + 127) / 128);
-        hipLaunchKernelGGL((k_kv4_weights<FMT, NG, T>),
-                           dim3(wgs, (unsigned)a.c.n_kv, (unsigned)a.s.n_seq), dim3(256), 0, st,
-                           a);
+        // eight blocks a wave (8 sequences to 8192 tokens: 2 blocks 56 us with the attention, 4
+        // 54, 8 52.5, 16 63), or one a workgroup
+        const int per = a.few ? 1024 : 64;
+        const dim3 grid((unsigned)a.c.n_kv, (unsigned)a.s.n_seq,
+                        (unsigned)std::min(65535, (max_len + per - 1) / per));
+        if (a.few)
+            hipLaunchKernelGGL((k_kv4_weights<FMT, NG, T, true>), grid, dim3(256), 0, st, a);
+        else
+            hipLaunchKernelGGL((k_kv4_weights<FMT, NG, T, false>), grid, dim3(256), 0, st, a);
         e = hipGetLastError();
     }
     return e;

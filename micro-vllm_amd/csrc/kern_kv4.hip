@@ -360,7 +360,8 @@ __device__ __forceinline__ uint32_t evict_key(float w) {
 // again in each pass.
 __global__ __launch_bounds__(1024) void k_kv4_select(EvictArgs A, int kcap) {
     extern __shared__ uint32_t keys[];
-    __shared__ uint32_t hist[2048];
+    __shared__ uint32_t hist[2][2048];  // of the even and the odd lanes: keys crowd in few bins
+    __shared__ uint32_t part[16];
     __shared__ int above[16], same[16];
     __shared__ uint32_t found[2];
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -382,45 +383,59 @@ __global__ __launch_bounds__(1024) void k_kv4_select(EvictArgs A, int kcap) {
         return phys < 0 ? 0u : evict_key(A.c.score[kv4_row(A.c, phys, h, t - pg * A.c.page)]);
     };
     const bool held = old <= kcap;
-    if (held)
-        for (int t = tid; t < old; t += 1024)
-            keys[t] = key_of(t);
+    if (held) {
+        // sixteen at a time: their table entries, then their scores, are on their way together
+        for (int t = tid; t < old; t += 16384) {
+            int pg[16], phys[16];
+            float w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                pg[i] = kv4_page_of(A.c, min(t + 1024 * i, old - 1));
+                phys[i] = kv4_phys(A.c, row, A.max_pages, pg[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                w[i] = A.c.score[kv4_row(A.c, max(phys[i], 0), h,
+                                         min(t + 1024 * i, old - 1) - pg[i] * A.c.page)];
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (t + 1024 * i < old)
+                    keys[t + 1024 * i] = phys[i] < 0 ? 0u : evict_key(w[i]);
+        }
+    }
     uint32_t prefix = 0, mask = 0;
     uint32_t want = (uint32_t)pick;  // of the keys that share the prefix
     if (pick > 0) {
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-            for (int i = tid; i < 2048; i += 1024)
-                hist[i] = 0;
+            hist[0][tid] = hist[0][tid + 1024] = hist[1][tid] = hist[1][tid + 1024] = 0;
             __syncthreads();
             for (int t = tid; t < old; t += 1024) {
                 const uint32_t key = held ? keys[t] : key_of(t);
                 if ((key & mask) == prefix)
-                    atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1)], 1u);
+                    atomicAdd(&hist[lane & 1][(key >> shift) & ((1u << bits) - 1)], 1u);
             }
             __syncthreads();
-            if (wave == 0) {  // 32 bins a lane, from the top
-                uint32_t sum = 0;
-                for (int i = 0; i < 32; ++i)
-                    sum += hist[2047 - (lane * 32 + i)];
-                uint32_t upto = sum;
-                for (int o = 1; o < 64; o <<= 1) {
-                    const uint32_t y = __shfl_up(upto, o);
-                    if (lane >= o)
-                        upto += y;
-                }
-                uint32_t before = upto - sum;
-                if (before < want && want <= upto) {
-                    for (int i = 0; i < 32; ++i) {
-                        const int bin = 2047 - (lane * 32 + i);
-                        const uint32_t c = hist[bin];
-                        if (before < want && want <= before + c) {
-                            found[0] = (uint32_t)bin;
-                            found[1] = want - before;
-                        }
-                        before += c;
-                    }
-                }
+            // two bins a thread, from the top
+            const int bin = 2047 - 2 * tid;
+            const uint32_t c0 = hist[0][bin] + hist[1][bin];
+            const uint32_t c1 = hist[0][bin - 1] + hist[1][bin - 1];
+            uint32_t upto = c0 + c1;
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t y = __shfl_up(upto, o);
+                if (lane >= o)
+                    upto += y;
+            }
+            if (lane == 63)
+                part[wave] = upto;
+            __syncthreads();
+            for (int w = 0; w < wave; ++w)
+                upto += part[w];
+            const uint32_t before = upto - c0 - c1;
+            if (before < want && want <= upto) {
+                const bool first = want <= before + c0;
+                found[0] = (uint32_t)(first ? bin : bin - 1);
+                found[1] = want - before - (first ? 0u : c0);
             }
             __syncthreads();
             prefix |= found[0] << shift;
@@ -467,19 +482,21 @@ __global__ __launch_bounds__(1024) void k_kv4_select(EvictArgs A, int kcap) {
         kept[pick + j] = old + j;
 }
 
-// One workgroup: 16 slots of one head of one sequence's fresh pages.  The kept rows' codes
-// move in 16-byte pieces, scales and weights after them.
+// One workgroup: 64 slots of one head of one sequence's fresh pages.  The kept rows' codes move
+// in 16-byte pieces, scales and scores after them, each thread's loads all on their way before
+// its first store.
 template <int FMT, int D>
 __global__ __launch_bounds__(256) void k_kv4_move(EvictArgs A) {
-    constexpr int CP = D / 32;                              // 16-byte pieces of a row's codes
-    constexpr int SB = FMT == 4 ? D / 16 : D / 32;          // bytes of a row's scales
-    constexpr int SU = FMT == 4 ? 4 : 2, SP = SB / SU;      // their pieces
-    __shared__ long long from[16], to[16];
-    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, j0 = blockIdx.x * 16;
+    constexpr int CP = D / 32;                          // 16-byte pieces of a row's codes
+    constexpr int SB = FMT == 4 ? D / 16 : D / 32;      // bytes of a row's scales
+    constexpr int SU = FMT == 4 ? 4 : 2, SP = SB / SU;  // their pieces
+    constexpr int NC = 2 * CP / 4, NS = (2 * SP + 1 + 3) / 4;  // pieces of a thread
+    __shared__ long long from[64], to[64];
+    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, j0 = blockIdx.x * 64;
     const int n = min(kv4_len(A.c, A.lens[b], A.max_pages), A.keep);
     if (j0 >= n)
         return;
-    if (tid < 16) {
+    if (tid < 64) {
         const int j = j0 + tid;
         long long f = -1, t = -1;
         if (j < n) {
@@ -497,37 +514,62 @@ __global__ __launch_bounds__(256) void k_kv4_move(EvictArgs A) {
         to[tid] = t;
     }
     __syncthreads();
-    for (int i = tid; i < 16 * 2 * CP; i += 256) {
+    u32x4 code[NC];
+    uint32_t rest[NS];
+    // piece i of the codes: its place in the pools' rows
+    auto codes_at = [&](int i, const long long *rows, uint8_t *&pool, long long &o) {
         const int r = i / (2 * CP), p = i - r * 2 * CP;
-        const long long f = from[r], t = to[r];
-        if (f < 0)
-            continue;
-        uint8_t *pool = p < CP ? A.c.k : A.c.v;
-        const int o = p < CP ? p : p - CP;
-        reinterpret_cast<uint4 *>(pool)[t * CP + o] = reinterpret_cast<const uint4 *>(pool)[f * CP + o];
-    }
-    for (int i = tid; i < 16 * (2 * SP + 1); i += 256) {
+        pool = p < CP ? A.c.k : A.c.v;
+        o = rows[r] < 0 ? -1 : rows[r] * CP + (p < CP ? p : p - CP);
+    };
+    auto rest_at = [&](int i, const long long *rows, uint8_t *&pool, long long &o, bool &score) {
         const int r = i / (2 * SP + 1), p = i - r * (2 * SP + 1);
-        const long long f = from[r], t = to[r];
-        if (f < 0)
-            continue;
-        if (p == 2 * SP) {
-            A.c.score[t] = A.c.score[f];
-            continue;
-        }
-        uint8_t *pool = p < SP ? A.c.ks : A.c.vs;
-        const int o = p < SP ? p : p - SP;
-        if constexpr (SU == 4)
-            reinterpret_cast<uint32_t *>(pool)[t * SP + o] =
-                reinterpret_cast<const uint32_t *>(pool)[f * SP + o];
+        const long long at = r < 64 ? rows[r & 63] : -1;
+        score = p == 2 * SP;
+        pool = p < SP ? A.c.ks : A.c.vs;
+        o = at < 0 ? -1 : score ? at : at * SP + (p < SP ? p : p - SP);
+    };
+    uint8_t *pool;
+    long long o;
+    bool score;
+#pragma unroll
+    for (int u = 0; u < NC; ++u) {
+        codes_at(tid + 256 * u, from, pool, o);
+        code[u] = reinterpret_cast<const u32x4 *>(pool)[max(o, 0ll)];
+    }
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {
+        rest_at(tid + 256 * u, from, pool, o, score);
+        o = max(o, 0ll);
+        if (score)
+            rest[u] = __float_as_uint(A.c.score[o]);
+        else if (SU == 4)
+            rest[u] = reinterpret_cast<const uint32_t *>(pool)[o];
         else
-            reinterpret_cast<uint16_t *>(pool)[t * SP + o] =
-                reinterpret_cast<const uint16_t *>(pool)[f * SP + o];
+            rest[u] = reinterpret_cast<const uint16_t *>(pool)[o];
+    }
+#pragma unroll
+    for (int u = 0; u < NC; ++u) {
+        codes_at(tid + 256 * u, to, pool, o);
+        if (o >= 0)
+            reinterpret_cast<u32x4 *>(pool)[o] = code[u];
+    }
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {
+        rest_at(tid + 256 * u, to, pool, o, score);
+        if (o >= 0) {
+            if (score)
+                A.c.score[o] = __uint_as_float(rest[u]);
+            else if (SU == 4)
+                reinterpret_cast<uint32_t *>(pool)[o] = rest[u];
+            else
+                reinterpret_cast<uint16_t *>(pool)[o] = (uint16_t)rest[u];
+        }
     }
 }
 
 // Keys that a selecting workgroup holds in LDS beside its histogram.
-constexpr int kEvictKeys = 36 * 1024;
+constexpr int kEvictKeys = 34 * 1024;
 
 hipError_t launch_kv4_evict(int fmt, int D, const EvictArgs &a, int max_len, hipStream_t st) {
     static const hipError_t lds = hipFuncSetAttribute(
@@ -543,7 +585,7 @@ hipError_t launch_kv4_evict(int fmt, int D, const EvictArgs &a, int max_len, hip
         return e;
     return kv4_by_shape(fmt, KV4_F32, D, [&](auto fm, auto, auto d) {
         hipLaunchKernelGGL((k_kv4_move<fm.value, d.value>),
-                           dim3((unsigned)((a.keep + 15) / 16), (unsigned)a.c.n_kv,
+                           dim3((unsigned)((a.keep + 63) / 64), (unsigned)a.c.n_kv,
                                 (unsigned)a.n_seq),
                            dim3(256), 0, st, a);
     });

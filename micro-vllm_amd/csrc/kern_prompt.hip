@@ -368,8 +368,8 @@ __global__ __launch_bounds__(64 * W, NG <= 2 ? 2 : 1) void k_kv4_prompt(AttnArgs
         const int last = min(rows, base + 32 * W) - 1;
         const int hi = max(0, min(pos0 + last / A.group + 1, len));
         const int lo = A.window > 0 ? max(0, min(pos0 + base / A.group - A.window + 1, hi)) : 0;
-        const int s0 = max(lo & ~(KT - 1), split * A.chunk);
-        const int s1 = split + 1 == A.splits ? hi : min(hi, (split + 1) * A.chunk);
+        const int s0 = (lo & ~(KT - 1)) + split * A.chunk;
+        const int s1 = split + 1 == A.splits ? hi : min(hi, s0 + A.chunk);
         const int n_tiles = s1 > s0 ? (s1 - s0 + KT - 1) / KT : 0;
         Prompt<FMT, NG, T, W, LSE> P{A, L, A.s.table + (size_t)seq * A.s.max_pages, head, s0, s1, wave};
 
@@ -649,23 +649,18 @@ static hipError_t prompt(const AttnArgs &a, hipStream_t st) {
 }
 
 template <int FMT, typename T>
-static hipError_t prompt_dim(int D, int waves, const AttnArgs &a, hipStream_t st) {
-    if (waves == 8)
-        return D == 64 ? prompt<FMT, 1, T, 8>(a, st) : D == 128 ? prompt<FMT, 2, T, 8>(a, st)
-                                                                : hipErrorInvalidValue;
-    return D == 64    ? prompt<FMT, 1, T, 4>(a, st)
-           : D == 128 ? prompt<FMT, 2, T, 4>(a, st)
+static hipError_t prompt_dim(int D, const AttnArgs &a, hipStream_t st) {
+    return D == 64    ? prompt<FMT, 1, T, 8>(a, st)
+           : D == 128 ? prompt<FMT, 2, T, 8>(a, st)
            : D == 192 ? prompt<FMT, 3, T, 4>(a, st)
            : D == 256 ? prompt<FMT, 4, T, 4>(a, st)
                       : hipErrorInvalidValue;
 }
 
-hipError_t launch_kv4_prompt(int fmt, int D, int dtype, int waves, const AttnArgs &a,
-                             hipStream_t st) {
+hipError_t launch_kv4_prompt(int fmt, int D, int dtype, const AttnArgs &a, hipStream_t st) {
     if (dtype == KV4_BF16)
-        return fmt == 4 ? prompt_dim<4, __bf16>(D, waves, a, st)
-                        : prompt_dim<7, __bf16>(D, waves, a, st);
-    return fmt == 4 ? prompt_dim<4, float>(D, waves, a, st) : prompt_dim<7, float>(D, waves, a, st);
+        return fmt == 4 ? prompt_dim<4, __bf16>(D, a, st) : prompt_dim<7, __bf16>(D, a, st);
+    return fmt == 4 ? prompt_dim<4, float>(D, a, st) : prompt_dim<7, float>(D, a, st);
 }
 
 }  // namespace mvllm_hip

@@ -14,6 +14,7 @@
 namespace mvllm_hip {
 void set_error(const std::string &s);  // mvllm_hip.cpp: the text of mvllm_hip_last_error
 int ready_device();                    // mvllm_hip.cpp: the device of mvllm_hip_init, or -1
+int kv4_rows_option();                 // mvllm_hip.cpp: option "kv4_rows"
 
 namespace {
 
@@ -264,8 +265,9 @@ int mvllm_hip_kv4_attention_dev(const mvllm_kv4 *cache, int dtype, const void *q
         (weights != KV4_WEIGHTS_NONE && !cache->score))
         return refuse("kv4_attention_dev: weights is 0, 1 or 2, and the cache has a score array "
                       "where it is not 0");
-    const AttnPlan p = kv4_attention_plan(cache->fmt, dtype, D, a.c.n_kv, n_q, n_tok, n_seq,
-                                          max_new, max_len, weights != KV4_WEIGHTS_NONE);
+    const AttnPlan p = kv4_attention_plan(kv4_rows_option(), cache->fmt, dtype, D, a.c.n_kv, n_q, n_tok, n_seq,
+                                          max_new, max_len, window,
+                                          weights != KV4_WEIGHTS_NONE);
     const size_t need = kv4_attention_bytes(D, a.c.n_kv, n_q, n_tok, n_seq, max_new, max_len,
                                             weights != KV4_WEIGHTS_NONE);
     if (need > work_bytes || (need && (!work || !aligned16(work))))
@@ -284,6 +286,7 @@ int mvllm_hip_kv4_attention_dev(const mvllm_kv4 *cache, int dtype, const void *q
     a.chunk = p.chunk;
     a.tiles = p.tiles;
     a.waves = p.waves;
+    a.few = (long long)max_new * a.group <= 16;
     const double scale2 = (double)scale * 1.44269504088896340736;
     a.scale2 = (float)scale2;
     a.scale2_lo = (float)(scale2 - (double)a.scale2);

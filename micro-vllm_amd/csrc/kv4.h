@@ -52,6 +52,7 @@ struct AttnArgs {
     float *lse;    // [n_tok][n_q] log2 of a row's sum of exponentials (-inf: sees nothing), or null
     long long q_stride;
     int n_q, group, splits, chunk, tiles, waves;
+    bool few;  // at most 16 rows a sequence and kv head, by max_new
     float scale2, scale2_lo;  // scale * log2(e), and what the f32 leaves of it
     int window, weights;
 };
@@ -78,13 +79,13 @@ struct AttnPlan {
     int splits, chunk, tiles;
     size_t part, ml, lse, bytes;  // offsets into the workspace, and its size
 };
-AttnPlan kv4_attention_plan(int fmt, int dtype, int head_dim, int n_kv, int n_q, int n_tok,
-                            int n_seq, int max_new, int max_len, bool weights);
-// The workspace that serves every format and type.
+// choice: 0 by size, 1 the 16-row kernel, 2 the other.
+AttnPlan kv4_attention_plan(int choice, int fmt, int dtype, int head_dim, int n_kv, int n_q, int n_tok,
+                            int n_seq, int max_new, int max_len, int window, bool weights);
+// The workspace that serves every choice, format, type and window.
 size_t kv4_attention_bytes(int head_dim, int n_kv, int n_q, int n_tok, int n_seq, int max_new,
                            int max_len, bool weights);
-hipError_t launch_kv4_prompt(int fmt, int head_dim, int dtype, int waves, const AttnArgs &a,
-                             hipStream_t st);
+hipError_t launch_kv4_prompt(int fmt, int head_dim, int dtype, const AttnArgs &a, hipStream_t st);
 hipError_t launch_kv4_attention(int fmt, int head_dim, int dtype, const AttnArgs &a, int max_len,
                                 hipStream_t st);
 

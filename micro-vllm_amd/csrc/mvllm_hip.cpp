@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <chrono>
 #include <cstdint>
 #include <cstdio>
@@ -27,6 +28,7 @@
 namespace mvllm_hip {
 void set_error(const std::string &s);
 int ready_device();
+int kv4_rows_option();
 }
 
 using namespace mvllm_hip;
@@ -255,6 +257,7 @@ struct Ctx {
     int gemm = 0;            // grouped GEMM: 0 auto, 1 whenever it applies, 2 never
     int fp4act = 0;          // MXFP4 experts: 1 = quantize activations, native FP4 GEMMs
     int combine_ordered = 0;  // 1 = separate combine in the reference's order (decode too)
+    std::atomic<int> kv4_rows{0};  // many-row attention: 0 by size, 1 16-row kernel, 2 256-row
     int dec_inline = 1;      // decode: gate/up descriptors in the kernel arguments when they fit
     // residency
     size_t budget = size_t(64) << 30;
@@ -297,6 +300,7 @@ Ctx &ctx() {
 
 // the device of mvllm_hip_init, or -1 before it
 int mvllm_hip::ready_device() { return ctx().ready ? ctx().device : -1; }
+int mvllm_hip::kv4_rows_option() { return ctx().kv4_rows; }
 
 namespace {
 
@@ -1496,6 +1500,10 @@ int mvllm_hip_set_option(const char *key, long long value) {
         C.combine_ordered = value ? 1 : 0;
     } else if (k == "fp4act") {
         C.fp4act = value ? 1 : 0;
+    } else if (k == "kv4_rows") {
+        if (value < 0 || value > 2)
+            return 0;
+        C.kv4_rows = static_cast<int>(value);
     } else if (k == "gemm") {
         if (value < 0 || value > 2)
             return 0;

@@ -10,13 +10,16 @@ Bars, by the roundings that can meet (u = 2^-24, half an f32 step; h = 2^-8, hal
   of itself, a probability by ln 2 of that and 2 u, in numerator and denominator; the sums of n
   products add (n + 64) u of sum P |v|.  bf16: probabilities as two terms (h^2 / 2 of sum P |v|)
   and the output's own h.
-- attention of more than 48 rows of a kv head (f16 operands, f = 2^-12 half an f16 step): bf16
+- attention of more than 16 rows of a kv head (maybe f16 operands, f = 2^-12 half an f16 step): bf16
   calls round a probability once (f), an int4 scale and its product with a code once each, of
   keys (an exponent is off by 2 f of sum |q k|) and of values (2 f of sum P |v|); MXFP4 is exact.
   f32 calls hold each rounded operand in two terms (f^2 of it, 2^-24, taken as 2 u for its
   subnormal second terms) and leave out the product of the second two (f^2): 3 * 2 u of sum
   |q k| and of sum P |v|.  So do the exponents of calls that collect weights, whose own sums
-  take exact products.
+  take exact products.  Below 2^-14 an f16 holds steps of 2^-24: probabilities are carried so
+  that the largest is 2^7 (bf16; 2^14 f32) or more, so each of n is off by 2^-32 (2^-39) of
+  the row's sum at least, and a value by 2^-25 of 2^14 for the largest of its tile: n 2^-31
+  (2^-38) of the largest |v| beside the rest.
 - the 2-norm: errors of independent roundings grow as their root: exponents 4 u of the largest
   one, 16 u beside; f16 keys' 2 f of the root of the sum of (q k)^2, twice for the
   denominator's share; f16 values and probabilities 3 f.
@@ -228,13 +231,13 @@ def run_attention(hip, cache, dtype, q, q_start, lens, tab, max_new, max_len, sc
 
 
 def check_attention(c, q, got, score, q_start, lens, tab, scale, window, weights, dtype,
-                    fill=5.0):
+                    fill=5.0, forced=False):
     D = q.shape[2]
     out, mag, (top, sums, root), exp_score = kvref.attention(c, q, q_start, lens, tab, scale,
                                                              window, weights)
     own = ~np.isnan(out).all((1, 2))
     assert (got[~own] == fill).all()
-    prompt = int(np.max(np.diff(q_start))) * (q.shape[1] // c["k"].shape[1]) > 48
+    prompt = int(np.max(np.diff(q_start))) * (q.shape[1] // c["k"].shape[1]) > 16 or forced
     f = 2.0 ** -12 if prompt else 0.0
     k_off = (2 * f if c["fmt"] == 4 else 0) if dtype == "bf16" else 6 * U * prompt
     v_off = (3 * f if c["fmt"] == 4 else f) if dtype == "bf16" else 6 * U * prompt
@@ -243,6 +246,9 @@ def check_attention(c, q, got, score, q_start, lens, tab, scale, window, weights
         k_off = w_off
     p_off = 2 * (np.log(2) * (U * (D * sums + 2 * top) + k_off * sums) + 2 * U)
     tol = mag * (p_off + v_off + (max(max(lens), 1) + 64) * U)
+    if prompt:
+        vs = c["vs"].astype(np.float64) if c["fmt"] == 4 else 2.0 ** (c["vs"] - 127.0)
+        tol = tol + max(lens) * 2.0 ** (-31 if dtype == "bf16" else -38) * 8 * np.abs(vs).max()
     if dtype == "bf16":
         tol = tol + H * np.abs(out) + H * H / 2 * mag
     assert (np.abs(got - out)[own] <= tol[own] + 1e-37).all()
@@ -279,8 +285,16 @@ ATTN = [
 ]
 
 
+@pytest.fixture(params=[0, 2], ids=["by size", "many rows"])
+def rows_kernel(hip, request):
+    """The kernel by the call's size, and that of many rows at every size."""
+    assert hip.set_option("kv4_rows", request.param)
+    yield request.param
+    assert hip.set_option("kv4_rows", 0)
+
+
 @pytest.mark.parametrize("case", ATTN, ids=lambda c: "-".join(map(str, c[:6])))
-def test_attention(hip, case):
+def test_attention(hip, rows_kernel, case):
     fmt, dtype, Hq, Hkv, D, page, lens, news, window, weights = case
     rng = np.random.default_rng(sum(lens) + D + Hq + fmt)
     n_pages = sum(-(-n // page) for n in lens) + len(lens) * (max(lens) // page + 3)
@@ -292,7 +306,7 @@ def test_attention(hip, case):
     out = run_attention(hip, cache, dtype, q, dev(qs), dev(ln), dev(tab), max(news), max(lens),
                         D ** -0.5, window, weights)
     err = check_attention(c, host(q), host(out), host(arr["score"]), qs, ln, tab, D ** -0.5, window,
-                          weights, dtype)
+                          weights, dtype, forced=rows_kernel == 2)
     print("  err", err, flush=True)
     for n in ("k", "ks", "v", "vs"):
         assert np.array_equal(host(arr[n]), c[n])
@@ -303,7 +317,7 @@ def test_attention(hip, case):
 @pytest.mark.parametrize("fmt", [4, 7])
 @pytest.mark.parametrize("dtype,news,window", [("f32", [1, 1], 0), ("bf16", [20, 40], 0),
                                                ("f32", [1, 1], 30), ("bf16", [40, 20], 17)])
-def test_attention_ignores_what_is_not_seen(hip, fmt, dtype, news, window):
+def test_attention_ignores_what_is_not_seen(hip, rows_kernel, fmt, dtype, news, window):
     """Non-finite scales behind a sequence's end, on its unseen pages, behind bad table entries and
     ahead of every window change nothing; bad entries are tokens that are not there."""
     rng = np.random.default_rng(fmt + len(dtype) + window)
@@ -317,7 +331,8 @@ def test_attention_ignores_what_is_not_seen(hip, fmt, dtype, news, window):
     ln = np.array(lens, np.int32)
     args = (dtype, q, dev(qs), dev(ln), dev(tab), max(news), max(lens), 0.2, window, 2)
     out = run_attention(hip, cache, *args)
-    check_attention(c, host(q), host(out), host(arr["score"]), qs, ln, tab, 0.2, window, 2, dtype)
+    check_attention(c, host(q), host(out), host(arr["score"]), qs, ln, tab, 0.2, window, 2, dtype,
+                    forced=rows_kernel == 2)
     used = np.zeros((60, page), bool)
     for b, n in enumerate(lens):
         first = max(0, n - news[b] - window + 1) if window else 0
@@ -335,7 +350,7 @@ def test_attention_ignores_what_is_not_seen(hip, fmt, dtype, news, window):
 
 
 @pytest.mark.parametrize("fmt,dtype", [(4, "f32"), (7, "bf16")])
-def test_masked_future_tokens_may_be_anything(hip, fmt, dtype):
+def test_masked_future_tokens_may_be_anything(hip, rows_kernel, fmt, dtype):
     """New tokens whose scales are not finite are seen by the rows from them on, and by no row
     ahead of them."""
     rng = np.random.default_rng(fmt)
@@ -355,7 +370,7 @@ def test_masked_future_tokens_may_be_anything(hip, fmt, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-def test_nonfinite_queries_stay_in_their_rows(hip, dtype):
+def test_nonfinite_queries_stay_in_their_rows(hip, rows_kernel, dtype):
     rng = np.random.default_rng(9)
     c = make_cache(rng, 7, 2, 64, 16, 40)
     tab, qs = tables(rng, [200, 100], 16, 40), starts([30, 1])
@@ -373,7 +388,7 @@ def test_nonfinite_queries_stay_in_their_rows(hip, dtype):
 
 
 @pytest.mark.parametrize("max_new,max_len", [(1, 1), (3, 100), (200, 5000)])
-def test_attention_sizes_are_hints(hip, max_new, max_len):
+def test_attention_sizes_are_hints(hip, rows_kernel, max_new, max_len):
     """Bounds below or above the real sizes change the launch, not what is computed."""
     rng = np.random.default_rng(3)
     c = make_cache(rng, 4, 2, 128, 32, 60)
@@ -383,10 +398,11 @@ def test_attention_sizes_are_hints(hip, max_new, max_len):
     q = dev(rng.standard_normal((110, 4, 128)).astype(np.float32))
     out = run_attention(hip, cache, "f32", q, dev(qs), dev(ln), dev(tab), max_new, max_len, 0.1, 0,
                         2)
-    check_attention(c, host(q), host(out), host(arr["score"]), qs, ln, tab, 0.1, 0, 2, "f32")
+    check_attention(c, host(q), host(out), host(arr["score"]), qs, ln, tab, 0.1, 0, 2, "f32",
+                    forced=rows_kernel == 2)
 
 
-def test_attention_scales(hip):
+def test_attention_scales(hip, rows_kernel):
     """Negative and zero scales, and logits past the exponents' range."""
     rng = np.random.default_rng(4)
     c = make_cache(rng, 4, 1, 64, 16, 20)
@@ -395,7 +411,8 @@ def test_attention_scales(hip):
     q = dev(rng.standard_normal((3, 4, 64)).astype(np.float32))
     for scale in (0.0, -0.2, 30.0):
         out = run_attention(hip, cache, "f32", q, dev(qs), dev(ln), dev(tab), 3, 200, scale)
-        check_attention(c, host(q), host(out), None, qs, ln, tab, scale, 0, 0, "f32")
+        check_attention(c, host(q), host(out), None, qs, ln, tab, scale, 0, 0, "f32",
+                        forced=rows_kernel == 2)
 
 
 def test_shared_pages_and_streams(hip):
@@ -602,7 +619,7 @@ def test_prompt_decode_evict_decode(hip, fmt, dtype):
             score[pl[0], :, pl[1]] = 0
         out, mag, (top, _, root), score = kvref.attention(now, host(st["q"]), qs, held, tab,
                                                           128 ** -0.5, 0, 1)
-        f, k_off = (2.0 ** -12, 6 * U) if st is p else (0.0, 0.0)
+        f, k_off = (2.0 ** -12, 6 * U) if st is p else (0.0, 0.0)  # many rows, maybe f16
         tol = (4 * top + 16) * U + (H if dtype == "bf16" else 0) + 2 * k_off * root + 3 * f
         assert np.linalg.norm(host(st["out"]) - out) <= tol * np.linalg.norm(out)
         assert np.linalg.norm(host(st["arr"]["score"]) - score) <= \
@@ -665,7 +682,7 @@ def test_captured_step_replays(hip, fmt, dtype):
             assert torch.equal(a["arr"][n], b["arr"][n]), n
 
 
-def test_repeats_are_equal(hip):
+def test_repeats_are_equal(hip, rows_kernel):
     """The same call again gives the same bits, weights included (no sum depends on an order)."""
     rng = np.random.default_rng(2)
     c = make_cache(rng, 4, 2, 128, 64, 120)
