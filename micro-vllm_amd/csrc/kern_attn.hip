@@ -13,6 +13,8 @@ namespace mvllm_hip {
 
 namespace {
 
+typedef float fl2 __attribute__((ext_vector_type(2)));
+
 __device__ __forceinline__ f4v mfma(bf16x8 a, bf16x8 b, f4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -53,16 +55,27 @@ template <typename T> __device__ __forceinline__ float power(const AttnArgs &A, 
 // as does every row that an infinite query or probability is in.
 template <int T>
 __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&t)[T]) {
+    u32x4 w[T];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float r = x[i];
+    for (int i = 0; i < 4; ++i) {  // two at a time: one conversion, and two words to take off
+        float a = x[2 * i], b = x[2 * i + 1];
 #pragma unroll
         for (int k = 0; k < T; ++k) {
-            t[k][i] = (__bf16)r;
-            if (k + 1 < T)
-                r -= (float)t[k][i];
+            const uint32_t u = as_u32(__builtin_convertvector(fl2{a, b}, bf16x2));
+            w[k][i] = u;
+            a -= __uint_as_float(u << 16);
+            b -= __uint_as_float(u & 0xffff0000u);
         }
     }
+#pragma unroll
+    for (int k = 0; k < T; ++k)
+        t[k] = __builtin_bit_cast(bf16x8, w[k]);
+}
+
+// row / group and row % group by a multiplication: with M = floor(2^40 / g) + 1, row * M >> 40 is
+// the quotient for row < 2^30 and g <= 1024 (M g exceeds 2^40 by at most g).
+__device__ __forceinline__ int token_of(const AttnArgs &A, int row) {
+    return (int)(((unsigned long long)(unsigned)row * A.group_rcp) >> 40);
 }
 
 // What a workgroup works on: one tile of 16 rows of one sequence and kv head.
@@ -91,7 +104,7 @@ __device__ __forceinline__ Tile tile_of(const AttnArgs &A, int seq, int head) {
 // The tokens that rows [r0, r1) may see: [lo, hi).
 __device__ __forceinline__ void span_of(const AttnArgs &A, const Tile &t, int r0, int r1, int &lo,
                                         int &hi) {
-    const int p0 = t.pos0 + r0 / A.group, p1 = t.pos0 + (r1 - 1) / A.group;
+    const int p0 = t.pos0 + token_of(A, r0), p1 = t.pos0 + token_of(A, r1 - 1);
     hi = max(0, min(p1 + 1, kv4_len(A.c, t.len, A.s.max_pages)));
     lo = A.window > 0 ? max(0, min(p0 - A.window + 1, hi)) : 0;
 }
@@ -104,8 +117,8 @@ template <int FMT, int NG, int TQ, typename T>
 __device__ __forceinline__ void load_q(const AttnArgs &A, const Tile &t, int row, bool live,
                                        bf16x8 (&q)[NG][2][TQ], float (&k8)[NG]) {
     const int kg = (threadIdx.x & 63) >> 4;
-    const int tok = t.first + (live ? row / A.group : 0);
-    const int head = t.head * A.group + (live ? row % A.group : 0);
+    const int i = live ? token_of(A, row) : 0, tok = t.first + i;
+    const int head = t.head * A.group + (live ? row - i * A.group : 0);
     const T *p = static_cast<const T *>(A.q) + (size_t)tok * A.q_stride +
                  (size_t)head * (64 * NG) + 16 * kg;
 #pragma unroll
@@ -480,11 +493,11 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
         const int s1 = split + 1 == A.splits ? hi : min(hi, s0 + A.chunk);
         const int row = r0 + col;
         const bool live = row < r1;
-        const int pos = t.pos0 + (live ? row : r0) / A.group;
+        const int pos = t.pos0 + token_of(A, live ? row : r0);
         const int from = A.window > 0 ? pos - A.window : -1;  // sees tokens above `from`
         // tokens that every row of the tile sees: [all0, all1)
-        const int all1 = min(s1, t.pos0 + r0 / A.group + 1);
-        const int all0 = A.window > 0 ? t.pos0 + (r1 - 1) / A.group - A.window + 1 : 0;
+        const int all1 = min(s1, t.pos0 + token_of(A, r0) + 1);
+        const int all0 = A.window > 0 ? t.pos0 + token_of(A, r1 - 1) - A.window + 1 : 0;
 
         Place at[2], ahead[2];
         Keys<FMT, NG> k[2];
@@ -504,6 +517,10 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
             for (int h = 0; h < 2; ++h)
                 v.load(A.c, kv4_row(A.c, max(at[h].phys, 0), t.head, at[h].slot), h);
         };
+        const int ri = live ? token_of(A, row) : 0;
+        const size_t logit_row =
+            ((size_t)(t.first + ri) * A.n_q + t.head * A.group + (live ? row - ri * A.group : 0)) *
+            (size_t)A.logits;
         const int b0 = s0 + 32 * wave;
         if (b0 < s1) {
             look(b0);
@@ -533,6 +550,9 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
                     s[4 * h + i] = y[i];
                     x[4 * h + i] = y[i] * A.scale2;
                 }
+                if (A.logit && live && t0 + 16 * h < A.logits)
+                    store4(A.logit + logit_row + t0 + 16 * h + 4 * kg,
+                           make_float4(y[0], y[1], y[2], y[3]));
             }
             if (more) {
                 at[0] = ahead[0];
@@ -541,6 +561,7 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
                 look(t0 + 256);
             }
             if (!(ok[0] && ok[1] && t0 >= all0 && t0 + 32 <= all1)) {
+                asm volatile("");  // a branch, not 70 selects in every block
                 uint32_t seen = 0;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -595,7 +616,8 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
         }
         __syncthreads();
         if (wave == 0 && live) {
-            const int tok = t.first + row / A.group, head = t.head * A.group + row % A.group;
+            const int i = token_of(A, row), tok = t.first + i;
+            const int head = t.head * A.group + row - i * A.group;
             const size_t at = ((size_t)split * A.s.n_tok + tok) * A.n_q + head;
             if (A.splits > 1) {
                 if (kg == 0)
@@ -627,10 +649,9 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
 // holds split s's maximum and sum (at most 64 splits), and groups of D / 8 lanes take every
 // other split's sums.
 template <int NG, typename T>
-__global__ __launch_bounds__(256) void k_kv4_join(AttnArgs A) {
+__device__ __forceinline__ void join(const AttnArgs &A, int tok, int head) {
     constexpr int D = 64 * NG, LPH = D / 8, G = 64 / LPH;
     const int lane = threadIdx.x & 63;
-    const int tok = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 6);
     if (head >= A.n_q || tok < A.s.q_start[0] || tok >= A.s.q_start[A.s.n_seq])
         return;
     const size_t at = (size_t)tok * A.n_q + head, step = (size_t)A.s.n_tok * A.n_q;
@@ -683,6 +704,124 @@ __global__ __launch_bounds__(256) void k_kv4_join(AttnArgs A) {
         A.lse[at] = L > 0.f ? M + log2f(L) : -INFINITY;
 }
 
+template <int NG, typename T>
+__global__ __launch_bounds__(256) void k_kv4_join(AttnArgs A) {
+    join<NG, T>(A, blockIdx.x, blockIdx.y * 4 + (threadIdx.x >> 6));
+}
+
+// The end of a decode call that collects weights, in one launch.  The first `joins` workgroups
+// join the splits, as above.  The others take 1024 tokens each of one sequence and kv head, four
+// a thread: the rows' maxima and sums from the splits', the tokens' logits as the attention
+// kernel left them (it has every key in its hands; reading its 4 bytes a row again costs less
+// than the key's codes and products: 8 sequences to 8192 tokens, groups of 4, 21 us with the
+// keys, 6 so).  Tokens past the logits' room (longer sequences than max_len) are multiplied out.
+template <int FMT, int NG, typename T>
+__global__ __launch_bounds__(256) void k_kv4_finish(AttnArgs A, int joins) {
+    constexpr int D = 64 * NG;
+    __shared__ float lse[16];
+    const int bx = blockIdx.x;
+    if (bx < joins) {
+        const int per = (A.n_q + 3) / 4;
+        join<NG, T>(A, bx / per, bx % per * 4 + (threadIdx.x >> 6));
+        return;
+    }
+    const int pair = (bx - joins) % (A.c.n_kv * A.s.n_seq), part = (bx - joins) / (A.c.n_kv * A.s.n_seq);
+    const int parts = ((int)gridDim.x - joins) / (A.c.n_kv * A.s.n_seq);
+    const Tile t = tile_of(A, pair / A.c.n_kv, pair % A.c.n_kv);
+    const int len = kv4_len(A.c, t.len, A.s.max_pages);
+    for (int r0 = 0; r0 < max(t.rows, 1); r0 += 16) {  // (more than 16 rows: max_new was less)
+        const int n_rows = min(16, t.rows - r0);
+        {
+            const int r = r0 + (threadIdx.x >> 4), j = threadIdx.x & 15;
+            const bool live = r < t.rows;
+            const int i = live ? token_of(A, r) : 0;
+            const size_t at = (size_t)(t.first + i) * A.n_q + t.head * A.group +
+                              (live ? r - i * A.group : 0);
+            if (A.splits == 1) {
+                if (j == 0)
+                    lse[threadIdx.x >> 4] = live ? A.lse[at] : -INFINITY;
+            } else {
+                const size_t step = (size_t)A.s.n_tok * A.n_q;
+                float2 ml[4];
+                float M = -INFINITY, L = 0.f;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int s = j + 16 * u;
+                    ml[u] = live && s < A.splits ? A.ml[at + s * step] : make_float2(-INFINITY, 0.f);
+                    M = fmaxf(M, ml[u].x);
+                }
+#pragma unroll
+                for (int o = 8; o >= 1; o >>= 1)
+                    M = fmaxf(M, __shfl_xor(M, o));
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    L += ml[u].y * (M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[u].x - M));
+                L = row_sum(L);
+                if (j == 0)
+                    lse[threadIdx.x >> 4] = L > 0.f || L != L ? M + log2f(L) : -INFINITY;
+            }
+        }
+        __syncthreads();
+        for (int t0 = (part * 256 + (int)threadIdx.x) * 4; t0 < len; t0 += parts * 1024) {
+            const int pg = kv4_page_of(A.c, t0);
+            const int phys = kv4_phys(A.c, t.table, A.s.max_pages, pg);
+            if (phys < 0)
+                continue;
+            const size_t place = kv4_row(A.c, phys, t.head, t0 - pg * A.c.page);
+            float w[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int n = 0; n < n_rows; ++n) {
+                const int r = r0 + n, i = token_of(A, r), pos = t.pos0 + i;
+                const int head = t.head * A.group + r - i * A.group;
+                const int from = A.window > 0 ? pos - A.window : -1;
+                if (t0 > pos || t0 + 3 <= from)
+                    continue;
+                float s[4];
+                if (t0 < A.logits) {
+                    const float4 y = *reinterpret_cast<const float4 *>(
+                        A.logit + ((size_t)(t.first + i) * A.n_q + head) * (size_t)A.logits + t0);
+                    s[0] = y.x; s[1] = y.y; s[2] = y.z; s[3] = y.w;
+                } else {
+                    const T *q = static_cast<const T *>(A.q) + (size_t)(t.first + i) * A.q_stride +
+                                 (size_t)head * D;
+#pragma unroll 1
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t *k =
+                            reinterpret_cast<const uint32_t *>(A.c.k) + (place + e) * (D / 8);
+                        float sum = 0.f;
+#pragma unroll 1
+                        for (int d = 0; d < D; d += 8) {
+                            const float sc =
+                                FMT == 4 ? reinterpret_cast<const float *>(
+                                               A.c.ks)[(place + e) * NG + d / 64]
+                                         : ue8m0_ref(A.c.ks[(place + e) * (2 * NG) + d / 32]);
+                            const uint32_t c = k[d / 8];
+                            float part = 0.f;
+#pragma unroll
+                            for (int z = 0; z < 8; ++z) {
+                                const uint32_t x = (c >> (4 * z)) & 15u;
+                                part = fmaf((float)q[d + z],
+                                            FMT == 4 ? (float)((int)x - 8) : e2m1_val(x), part);
+                            }
+                            sum = fmaf(part, sc, sum);
+                        }
+                        s[e] = sum;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (t0 + e <= pos && t0 + e > from)
+                        w[e] += power<T>(A, s[e], lse[n]);
+            }
+            float *p = A.c.score + place;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (t0 + e < len)
+                    p[e] = A.weights == KV4_WEIGHTS_ADD || r0 > 0 ? p[e] + w[e] : w[e];
+        }
+        __syncthreads();
+    }
+}
+
 // The weights of blocks of 16 NB tokens of one sequence and kv head, over all of its rows.  The
 // keys stay in registers as operands while the rows pass by, 16 at a time, and each token's sum
 // is formed in one place, in one order.
@@ -705,10 +844,10 @@ __global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs A) {
     auto rows_at = [&](int r) {
         row = r + col;
         live = row < t.rows;
-        pos = t.pos0 + (live ? row : 0) / A.group;
+        const int i = live ? token_of(A, row) : 0;
+        pos = t.pos0 + i;
         from = A.window > 0 ? pos - A.window : -1;
-        lse = live ? A.lse[(size_t)(t.first + row / A.group) * A.n_q + t.head * A.group +
-                           row % A.group]
+        lse = live ? A.lse[(size_t)(t.first + i) * A.n_q + t.head * A.group + row - i * A.group]
                    : -INFINITY;
         load_q<FMT, NG, TQ, T>(A, t, row, live, q, k8);
     };
@@ -854,6 +993,12 @@ static AttnPlan plan_for(bool prompt, int fmt, int dtype, int head_dim, int n_kv
     }
     if (weights)
         p.lse = add(heads * 4);
+    // decode keeps its logits for the weights, up to half a gigabyte of them
+    const size_t logits = ((size_t)max_len + 127) / 128 * 128;
+    if (weights && rows <= 16 && heads * logits * 4 <= (size_t(1) << 29)) {
+        p.logits = (int)logits;
+        p.logit = add(heads * logits * 4);
+    }
     return p;
 }
 
@@ -902,6 +1047,14 @@ static hipError_t attention(const AttnArgs &a, int max_len, hipStream_t st) {
     hipLaunchKernelGGL((k_kv4_attn<FMT, NG, T>), grid, dim3(256), 0, st, a);
     if ((e = hipGetLastError()) != hipSuccess)
         return e;
+    }
+    if (a.logit && !a.waves) {
+        const int pairs = a.c.n_kv * a.s.n_seq;
+        const int joins = a.splits > 1 ? a.s.n_tok * ((a.n_q + 3) / 4) : 0;
+        const int parts = std::max(1, std::min((max_len + 1023) / 1024, (1 << 24) / pairs));
+        hipLaunchKernelGGL((k_kv4_finish<FMT, NG, T>), dim3((unsigned)(joins + parts * pairs)),
+                           dim3(256), 0, st, a, joins);
+        return hipGetLastError();
     }
     if (a.splits > 1) {
         hipLaunchKernelGGL((k_kv4_join<NG, T>),

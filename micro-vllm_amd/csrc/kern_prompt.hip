@@ -489,6 +489,7 @@ __global__ __launch_bounds__(64 * W, NG <= 2 ? 2 : 1) void k_kv4_prompt(AttnArgs
                 const bool whole = t0 >= all0 && t0 + KT <= all1 && I.there[0] == ~0u &&
                                    I.there[1] == full;
                 if (!whole) {
+                    asm volatile("");  // a branch, not selects in every tile
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
 #pragma unroll

@@ -227,7 +227,7 @@ int mvllm_hip_kv4_read_dev(const mvllm_kv4 *cache, int dtype, void *k, void *v, 
 static bool attention_sizes_ok(int head_dim, int n_kv, int n_q, int n_tok, int n_seq, int max_new,
                                int max_len) {
     return head_dim_ok(head_dim) && n_kv >= 1 && n_kv <= 1024 && n_q >= n_kv && n_q % n_kv == 0 &&
-           n_q <= 65535 && n_tok >= 1 && n_seq >= 1 && n_seq <= 65535 && max_new >= 1 &&
+           n_q <= 65535 && n_q / n_kv <= 1024 && n_tok >= 1 && n_seq >= 1 && n_seq <= 65535 && max_new >= 1 &&
            max_len >= 1 && max_len <= (1 << 30) && (long long)n_tok * n_q <= (1ll << 30) &&
            (long long)max_new * n_q <= (1ll << 30);
 }
@@ -257,7 +257,7 @@ int mvllm_hip_kv4_attention_dev(const mvllm_kv4 *cache, int dtype, const void *q
         !std::isfinite(scale) || window < 0 ||
         ranges_meet(q, rows_bytes(dtype, n_tok, q_stride, (long long)n_q * D), out,
                     rows_bytes(dtype, n_tok, (long long)n_q * D, (long long)n_q * D)))
-        return refuse("kv4_attention_dev: bad arguments (dtype 0 or 1, n_q a multiple of n_kv, "
+        return refuse("kv4_attention_dev: bad arguments (dtype 0 or 1, n_q a multiple of n_kv up to 1024 times it, "
                       "16-byte aligned q and out that do not overlap, max_new >= 1, 1 <= max_len "
                       "<= 2^30, n_tok * n_q and max_new * n_q up to 2^30, finite scale, window >= "
                       "0)");
@@ -279,6 +279,9 @@ int mvllm_hip_kv4_attention_dev(const mvllm_kv4 *cache, int dtype, const void *q
     a.part = reinterpret_cast<float *>(w + p.part);
     a.ml = reinterpret_cast<float2 *>(w + p.ml);
     a.lse = weights != KV4_WEIGHTS_NONE ? reinterpret_cast<float *>(w + p.lse) : nullptr;
+    a.logit = p.logits && !p.waves ? reinterpret_cast<float *>(w + p.logit) : nullptr;
+    a.logits = p.logits;
+    a.group_rcp = (1ull << 40) / (unsigned)(n_q / a.c.n_kv) + 1;
     a.q_stride = q_stride;
     a.n_q = n_q;
     a.group = n_q / a.c.n_kv;

@@ -50,6 +50,9 @@ struct AttnArgs {
     float *part;   // [splits][n_tok][n_q][D] sums relative to the split's maximum
     float2 *ml;    // [splits][n_tok][n_q] maximum (log2) and sum of a split
     float *lse;    // [n_tok][n_q] log2 of a row's sum of exponentials (-inf: sees nothing), or null
+    float *logit;  // [n_tok][n_q][logits] products of queries and keys, or null
+    int logits;
+    unsigned long long group_rcp;  // floor(2^40 / group) + 1
     long long q_stride;
     int n_q, group, splits, chunk, tiles, waves;
     bool few;  // at most 16 rows a sequence and kv head, by max_new
@@ -77,7 +80,8 @@ hipError_t launch_kv4_evict(int fmt, int head_dim, const EvictArgs &a, int max_l
 struct AttnPlan {
     int waves;  // 0: 16 rows a workgroup, else 32 a wave
     int splits, chunk, tiles;
-    size_t part, ml, lse, bytes;  // offsets into the workspace, and its size
+    int logits;           // logits kept of each row (0: none)
+    size_t part, ml, lse, logit, bytes;  // offsets into the workspace, and its size
 };
 // choice: 0 by size, 1 the 16-row kernel, 2 the other.
 AttnPlan kv4_attention_plan(int choice, int fmt, int dtype, int head_dim, int n_kv, int n_q, int n_tok,
