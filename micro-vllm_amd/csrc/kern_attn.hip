@@ -503,9 +503,12 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
         Keys<FMT, NG> k[2];
         V v;
         auto look = [&](int t0) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                ahead[h] = place_of(A, t, t0 + 16 * h);
+            ahead[0] = place_of(A, t, t0);
+            ahead[1] = {ahead[0].phys, ahead[0].slot + 16};
+            if (A.c.page & 16) {  // else 32 tokens lie in one page
+                asm volatile("");
+                ahead[1] = place_of(A, t, t0 + 16);
+            }
         };
         auto fetch_keys = [&] {
 #pragma unroll
