@@ -146,24 +146,23 @@ template <int FMT, int NG> struct Keys {
     float s[FMT == 4 ? 4 * NG : NG];
 
     __device__ __forceinline__ void load(const Kv4View &c, size_t row) {
-        const int lane = threadIdx.x & 63, m = lane & 15, kg = lane >> 4;
-        const uint8_t *p = c.k + (row + m) * (32 * NG) + 8 * kg;
+        // (a base that the wave shares, and a lane's offset)
+        const uint32_t lane = threadIdx.x & 63, m = lane & 15, kg = lane >> 4;
+        const uint8_t *p = c.k + row * (32 * NG), *sp = c.ks + row * (FMT == 4 ? 4 * NG : 2 * NG);
 #pragma unroll
         for (int g = 0; g < NG; ++g)
-            w[g] = *reinterpret_cast<const uint2 *>(p + 32 * g);
+            w[g] = *reinterpret_cast<const uint2 *>(p + (m * (32 * NG) + 8 * kg + 32 * g));
         if constexpr (FMT == 4) {
-            const float4 *sp =
-                reinterpret_cast<const float4 *>(c.ks + (row + 4 * kg) * (4 * NG));
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const float4 v = sp[g];
+                const float4 v =
+                    *reinterpret_cast<const float4 *>(sp + (4 * kg * (4 * NG) + 16 * g));
                 s[4 * g] = v.x; s[4 * g + 1] = v.y; s[4 * g + 2] = v.z; s[4 * g + 3] = v.w;
             }
         } else {
-            const uint8_t *sp = c.ks + (row + m) * (2 * NG) + (kg >> 1);
 #pragma unroll
             for (int g = 0; g < NG; ++g)
-                s[g] = ue8m0_ref(sp[2 * g]);
+                s[g] = ue8m0_ref(sp[m * (2 * NG) + (kg >> 1) + 2 * g]);
         }
     }
 };
@@ -210,19 +209,17 @@ template <int NG, bool UNS> struct Vals<4, NG, UNS> {
     float s[8 * NG];  // [token][group]
 
     __device__ __forceinline__ void load(const Kv4View &c, size_t row, int half) {
-        const int lane = threadIdx.x & 63, m = lane & 15, kg = lane >> 4;
-        row += 4 * kg;
-        const uint8_t *p = c.v + row * (32 * NG) + 2 * m;
+        const uint32_t lane = threadIdx.x & 63, m = lane & 15, kg = lane >> 4;
+        const uint8_t *p = c.v + row * (32 * NG), *sp = c.vs + row * (4 * NG);
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                w[g][4 * half + i] =
-                    *reinterpret_cast<const uint16_t *>(p + i * (32 * NG) + 32 * g);
-        const float4 *sp = reinterpret_cast<const float4 *>(c.vs + row * (4 * NG));
+                w[g][4 * half + i] = *reinterpret_cast<const uint16_t *>(
+                    p + ((4 * kg + i) * (32 * NG) + 32 * g + 2 * m));
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            const float4 v = sp[g];
+            const float4 v = *reinterpret_cast<const float4 *>(sp + (4 * kg * (4 * NG) + 16 * g));
             const int o = 4 * NG * half + 4 * g;
             s[o] = v.x; s[o + 1] = v.y; s[o + 2] = v.z; s[o + 3] = v.w;
         }
@@ -322,23 +319,22 @@ template <int NG, bool UNS> struct Vals<7, NG, UNS> {
     uint32_t b[2][2 * NG];  // scale bytes [token][2 NG] of 4 tokens
 
     __device__ __forceinline__ void load(const Kv4View &c, size_t row, int half) {
-        const int lane = threadIdx.x & 63, m = lane & 15, kg = lane >> 4;
-        row += 4 * kg;
-        const uint8_t *p = c.v + row * (32 * NG);
+        const uint32_t lane = threadIdx.x & 63, m = lane & 15, kg = lane >> 4;
+        const uint8_t *p = c.v + row * (32 * NG), *sp = c.vs + row * (2 * NG);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+            const uint32_t at = (4 * kg + i) * (32 * NG);
 #pragma unroll
             for (int n = 0; n < NC; ++n)
                 w[n][4 * half + i] =
-                    *reinterpret_cast<const uint32_t *>(p + i * (32 * NG) + 64 * n + 4 * m);
+                    *reinterpret_cast<const uint32_t *>(p + (at + 64 * n + 4 * m));
             if constexpr (ODD)
                 w[NC][4 * half + i] =
-                    *reinterpret_cast<const uint16_t *>(p + i * (32 * NG) + 64 * NC + 2 * m);
+                    *reinterpret_cast<const uint16_t *>(p + (at + 64 * NC + 2 * m));
         }
-        const uint2 *sp = reinterpret_cast<const uint2 *>(c.vs + row * (2 * NG));
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            const uint2 v = sp[g];
+            const uint2 v = *reinterpret_cast<const uint2 *>(sp + (4 * kg * (2 * NG) + 8 * g));
             b[half][2 * g] = v.x;
             b[half][2 * g + 1] = v.y;
         }
@@ -446,15 +442,28 @@ __device__ __forceinline__ void store4(__bf16 *p, float4 y) {
     *reinterpret_cast<uint2 *>(p) = make_uint2(as_u32(a), as_u32(b));
 }
 
-// Where 16 tokens from t0 on (a multiple of 16) lie: the pool page (-1: nowhere) and its slot.
+// Where 16 tokens from t0 on (a multiple of 16) lie: the cache's row of the first (page 0's where
+// there is none), and whether they are there.
 struct Place {
-    int phys, slot;
+    size_t row;
+    bool ok;
 };
-__device__ __forceinline__ Place place_of(const AttnArgs &A, const Tile &t, int t0) {
-    const int pg = kv4_page_of(A.c, t0);
-    return {__builtin_amdgcn_readfirstlane(kv4_phys(A.c, t.table, A.s.max_pages, pg)),
-            t0 - pg * A.c.page};
-}
+// A table entry on its way: loaded a block ahead and looked at only when it is needed (loads
+// come back in order, so a wave that looked at once would wait for the keys before it too).
+struct Entry {
+    int t0, pg, raw;
+
+    __device__ __forceinline__ void load(const AttnArgs &A, const Tile &t, int tok) {
+        t0 = tok;
+        pg = kv4_page_of(A.c, tok);
+        raw = t.table[min(pg, A.s.max_pages - 1)];
+    }
+    __device__ __forceinline__ Place place(const AttnArgs &A, const Tile &t) const {
+        const int phys = __builtin_amdgcn_readfirstlane(raw);
+        const bool ok = pg < A.s.max_pages && (unsigned)phys < (unsigned)A.c.n_pages;
+        return {kv4_row(A.c, ok ? phys : 0, t.head, t0 - pg * A.c.page), ok};
+    }
+};
 
 }  // namespace
 
@@ -499,26 +508,34 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
         const int all1 = min(s1, t.pos0 + token_of(A, r0) + 1);
         const int all0 = A.window > 0 ? t.pos0 + token_of(A, r1 - 1) - A.window + 1 : 0;
 
-        Place at[2], ahead[2];
+        Place at[2];
+        Entry ahead[2];
         Keys<FMT, NG> k[2];
         V v;
         auto look = [&](int t0) {
-            ahead[0] = place_of(A, t, t0);
-            ahead[1] = {ahead[0].phys, ahead[0].slot + 16};
+            ahead[0].load(A, t, t0);
             if (A.c.page & 16) {  // else 32 tokens lie in one page
                 asm volatile("");
-                ahead[1] = place_of(A, t, t0 + 16);
+                ahead[1].load(A, t, t0 + 16);
+            }
+        };
+        auto arrive = [&] {
+            at[0] = ahead[0].place(A, t);
+            at[1] = {at[0].row + 16, at[0].ok};
+            if (A.c.page & 16) {
+                asm volatile("");
+                at[1] = ahead[1].place(A, t);
             }
         };
         auto fetch_keys = [&] {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                k[h].load(A.c, kv4_row(A.c, max(at[h].phys, 0), t.head, at[h].slot));
+                k[h].load(A.c, at[h].row);
         };
         auto fetch_vals = [&] {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                v.load(A.c, kv4_row(A.c, max(at[h].phys, 0), t.head, at[h].slot), h);
+                v.load(A.c, at[h].row, h);
         };
         const int ri = live ? token_of(A, row) : 0;
         const size_t logit_row =
@@ -527,11 +544,10 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
         const int b0 = s0 + 32 * wave;
         if (b0 < s1) {
             look(b0);
-            at[0] = ahead[0];
-            at[1] = ahead[1];
+            arrive();
+            look(b0 + 128);
             fetch_keys();
             fetch_vals();
-            look(b0 + 128);
         }
         bf16x8 q[NG][2][TQ];
         float k8[NG];
@@ -542,7 +558,7 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
 
         for (int t0 = b0; t0 < s1; t0 += 128) {
             // a page that is none: its tokens are not there
-            const bool ok[2] = {at[0].phys >= 0, at[1].phys >= 0};
+            const bool ok[2] = {at[0].ok, at[1].ok};
             const bool more = t0 + 128 < s1;
             float s[8], x[8], p[8];
 #pragma unroll
@@ -558,10 +574,9 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
                            make_float4(y[0], y[1], y[2], y[3]));
             }
             if (more) {
-                at[0] = ahead[0];
-                at[1] = ahead[1];
-                fetch_keys();
+                arrive();
                 look(t0 + 256);
+                fetch_keys();
             }
             if (!(ok[0] && ok[1] && t0 >= all0 && t0 + 32 <= all1)) {
                 asm volatile("");  // a branch, not 70 selects in every block
@@ -858,11 +873,15 @@ __global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs A) {
     bool ok[NB];
     size_t at[NB];
     auto fetch = [&](int t0, Keys<FMT, NG> *to) {
+        Entry e[NB];
+#pragma unroll
+        for (int h = 0; h < NB; ++h)
+            e[h].load(A, t, t0 + 16 * h);
 #pragma unroll
         for (int h = 0; h < NB; ++h) {
-            const Place pl = place_of(A, t, t0 + 16 * h);
-            ok[h] = pl.phys >= 0;
-            at[h] = kv4_row(A.c, max(pl.phys, 0), t.head, pl.slot);
+            const Place pl = e[h].place(A, t);
+            ok[h] = pl.ok;
+            at[h] = pl.row;
             to[h].load(A.c, at[h]);
         }
     };
