@@ -18,7 +18,9 @@ namespace mvllm_hip {
 // elements each (NC blocks of them for D = 192), so its sum of squares is a butterfly within
 // the wave.  The token's cosines and sines are formed once per workgroup, in LDS: the angle in
 // 64 bits (pos up to 2^31 turns an f32 angle by radians), reduced by quarter turns to +-1/8
-// turn before it is rounded to f32, so far positions are as exact as near ones.
+// turn before it is rounded to f32, so far positions are as exact as near ones.  Bound by the
+// bytes: 4096 tokens, 72 heads of 128 in bf16 read and written in 33.6 us, 4.5 TB/s (a large
+// copy reaches 5.0).
 template <typename T, int D, bool INTER>
 __global__ __launch_bounds__(256) void k_qk_norm_rope(RopeArgs A) {
     constexpr int LPH = D == 64 || D == 192 ? 8 : D / 8, NC = D / 8 / LPH, HPW = 64 / LPH;
@@ -129,7 +131,11 @@ hipError_t launch_qk_norm_rope(int dtype, int n_tok, int D, bool interleaved, Ro
                                hipStream_t st) {
     const int per = 4 * (D == 64 || D == 192 ? 8 : 512 / D);  // heads of one pass of a workgroup
     const int total = a.n_q + a.n_kv;
-    a.heads_per_wg = per;
+    // All heads of a token in one workgroup, so that its angles are formed once (4096 tokens, 72
+    // heads of 128 in bf16: 33.6 us, and 36.7 with a workgroup for each pass), unless that leaves
+    // fewer than 2048 workgroups (16 tokens: one pass each, 3.6 us).
+    const long long parts = (total + per - 1) / per;
+    a.heads_per_wg = per * (int)std::max(1ll, std::min(parts, n_tok * parts / 2048));
     const dim3 grid((unsigned)n_tok, (unsigned)((total + a.heads_per_wg - 1) / a.heads_per_wg));
     if (dtype == KV4_BF16)
         return interleaved ? rope_dim<__bf16, true>(n_tok, D, a, grid, st)
@@ -187,7 +193,10 @@ __device__ __forceinline__ uint32_t kv4_e2m1(float q) {
 // One wave: 64 blocks of 8 elements of one token's keys (grid y 0) or values (y 1); a group's
 // largest magnitude is a butterfly over its 8 (int4) or 4 (MXFP4) lanes.  The wave's first
 // loads are its elements and the sequences' ends and lengths, one round trip; the table
-// entry is the second, then it stores.
+// entry is the second, then it stores.  Few tokens are bound by those two trips and the launch
+// (16 tokens, 8 heads of 128: 4.0 us), many by their stores of 4 bytes a lane (4096 tokens, 8
+// heads of 128 in bf16, 22 MB: 12.9 us, 1.7 TB/s; a wave with two heads in flight took 13.9,
+// one with four tokens of four heads, a page's rows side by side, 14.5).
 template <int FMT, typename T, int D>
 __global__ __launch_bounds__(256) void k_kv4_append(Kv4View C, Kv4Seqs S, const T *k,
                                                     long long k_stride, const T *v,

@@ -139,7 +139,12 @@ def set_option(key: str, value: int) -> bool:
     return lib().mvllm_hip_set_option(key.encode(), int(value)) == 1
 
 
+_Tensor = None if torch is None else torch.Tensor
+
+
 def _ptr(a):
+    if type(a) is _Tensor:  # first: a call has up to ten of them
+        return a.data_ptr()
     if a is None or isinstance(a, int):  # an address the caller already holds
         return a
     if isinstance(a, np.ndarray):
