@@ -303,7 +303,8 @@ int mvllm_hip_rmsnorm_dev(const float *x, const float *w, float *y, int rows, in
  * lens[b].  Rows ahead of q_start[0] or behind q_start[n_seq] belong to no sequence and are
  * left as they are.  A table entry outside [0, n_pages), or a token past the table, is a token
  * that is not there: not written, not seen, read as zeros.  A row whose token would be before
- * its sequence's first (more rows than lens[b]) has no place in the cache. */
+ * its sequence's first (more rows than lens[b]) has no place in the cache.  n_tok is at most
+ * 2^23, n_tok * n_kv * head_dim at most 2^34, max_pages * page at most 2^30. */
 typedef struct mvllm_kv4 {
     void *k, *ks, *v, *vs;
     float *score;
@@ -385,7 +386,8 @@ long long mvllm_hip_kv4_attention_work(int n_kv, int head_dim, int n_q, int n_to
  * it).  The source pages are left as they are; a moved token that is not there leaves its
  * place as it is.  Positions: a cached key keeps its rotation; the engine goes on counting
  * positions for new tokens, while lens, causality and windows count the tokens held.
- * max_len: the most tokens the launch is sized for; longer sequences run too, slower. */
+ * max_len: the most tokens the launch is sized for; longer sequences run too, slower.  A length
+ * past the table counts as the table's end here; keep is at most 2^29. */
 int mvllm_hip_kv4_evict_dev(const mvllm_kv4 *cache, const int *lens, const int *table, int n_seq,
                             int max_pages, int max_len, int keep, int recent,
                             const int *dst_table, int dst_max_pages, int *kept, int *new_lens,

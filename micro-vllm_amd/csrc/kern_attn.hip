@@ -101,12 +101,13 @@ __device__ __forceinline__ Tile tile_of(const AttnArgs &A, int seq, int head) {
     return t;
 }
 
-// The tokens that rows [r0, r1) may see: [lo, hi).
+// The tokens that rows [r0, r1) may see: [lo, hi).  (A row ahead of the sequence's first token
+// moves neither, and its position no difference past 32 bits.)
 __device__ __forceinline__ void span_of(const AttnArgs &A, const Tile &t, int r0, int r1, int &lo,
                                         int &hi) {
     const int p0 = t.pos0 + token_of(A, r0), p1 = t.pos0 + token_of(A, r1 - 1);
     hi = max(0, min(p1 + 1, kv4_len(A.c, t.len, A.s.max_pages)));
-    lo = A.window > 0 ? max(0, min(p0 - A.window + 1, hi)) : 0;
+    lo = A.window > 0 ? max(0, min(max(p0, 0) - A.window + 1, hi)) : 0;
 }
 
 // B operands of 16 rows of queries: lane (column c, group of lanes kg) holds, of each 64
@@ -469,7 +470,9 @@ struct Entry {
 
 // Waves a SIMD whose registers hold an attention kernel without spilling.
 constexpr int attn_waves(int fmt, int ng, bool f32) {
-    return ng <= 2 && !f32 && (ng == 1 || fmt == 7) ? 3 : ng <= 2 || (ng == 3 && fmt == 7) || (fmt == 7 && !f32) ? 2 : 1;
+    if (ng <= 2)
+        return !f32 && (ng == 1 || fmt == 7) ? 3 : 2;
+    return fmt == 7 && (ng == 3 || !f32) ? 2 : 1;
 }
 
 // One workgroup: tiles of 16 rows of one sequence and kv head over one split of the tokens;
@@ -498,8 +501,8 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
         const int r1 = min(t.rows, r0 + 16);
         int lo, hi;
         span_of(A, t, r0, r1, lo, hi);
-        const int s0 = (lo & ~31) + split * A.chunk;
-        const int s1 = split + 1 == A.splits ? hi : min(hi, s0 + A.chunk);
+        const int s0 = (int)min((long long)hi, (lo & ~31) + (long long)split * A.chunk);
+        const int s1 = split + 1 == A.splits ? hi : min(hi - s0, A.chunk) + s0;
         const int row = r0 + col;
         const bool live = row < r1;
         const int pos = t.pos0 + token_of(A, live ? row : r0);
@@ -644,20 +647,21 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
                 A.lse[at] = L > 0.f ? M + log2f(L) : -INFINITY;
             }
             const float scale = A.splits > 1 ? 1.f : L > 0.f || L != L ? 1.f / L : 0.f;
-            if (A.splits == 1 || M != -INFINITY)  // (the join leaves a split of nothing out)
-            o.pieces(kg, [&](int d, float4 y) {
-                y = make_float4(y.x * fix, y.y * fix, y.z * fix, y.w * fix);
+            if (A.splits == 1 || M != -INFINITY) {  // (the join leaves a split of nothing out)
+                o.pieces(kg, [&](int d, float4 y) {
+                    y = make_float4(y.x * fix, y.y * fix, y.z * fix, y.w * fix);
 #pragma unroll
-                for (int w = 0; w < 3; ++w) {
-                    const float4 z = *reinterpret_cast<const float4 *>(&osum[w][col][d]);
-                    y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
-                }
-                y = make_float4(y.x * scale, y.y * scale, y.z * scale, y.w * scale);
-                if (A.splits > 1)
-                    *reinterpret_cast<float4 *>(A.part + at * D + d) = y;
-                else
-                    store4(static_cast<T *>(A.out) + ((size_t)tok * A.n_q + head) * D + d, y);
-            });
+                    for (int w = 0; w < 3; ++w) {
+                        const float4 z = *reinterpret_cast<const float4 *>(&osum[w][col][d]);
+                        y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+                    }
+                    y = make_float4(y.x * scale, y.y * scale, y.z * scale, y.w * scale);
+                    if (A.splits > 1)
+                        *reinterpret_cast<float4 *>(A.part + at * D + d) = y;
+                    else
+                        store4(static_cast<T *>(A.out) + ((size_t)tok * A.n_q + head) * D + d, y);
+                });
+            }
         }
         __syncthreads();
     }
@@ -743,8 +747,9 @@ __global__ __launch_bounds__(256) void k_kv4_finish(AttnArgs A, int joins) {
         join<NG, T>(A, bx / per, bx % per * 4 + (threadIdx.x >> 6));
         return;
     }
-    const int pair = (bx - joins) % (A.c.n_kv * A.s.n_seq), part = (bx - joins) / (A.c.n_kv * A.s.n_seq);
-    const int parts = ((int)gridDim.x - joins) / (A.c.n_kv * A.s.n_seq);
+    const int pairs = A.c.n_kv * A.s.n_seq;
+    const int pair = (bx - joins) % pairs, part = (bx - joins) / pairs;
+    const int parts = ((int)gridDim.x - joins) / pairs;
     const Tile t = tile_of(A, pair / A.c.n_kv, pair % A.c.n_kv);
     const int len = kv4_len(A.c, t.len, A.s.max_pages);
     for (int r0 = 0; r0 < max(t.rows, 1); r0 += 16) {  // (more than 16 rows: max_new was less)
@@ -1063,12 +1068,12 @@ static hipError_t attention(const AttnArgs &a, int max_len, hipStream_t st) {
             hipSuccess)
             return e;
     } else {
-    // Heads go round the XCDs first, splits last: sequences of unlike length leave the later
-    // splits empty, and with the splits first the XCDs that got those had nothing to do.
-    const dim3 grid((unsigned)a.c.n_kv, (unsigned)a.s.n_seq, (unsigned)(a.splits * a.tiles));
-    hipLaunchKernelGGL((k_kv4_attn<FMT, NG, T>), grid, dim3(256), 0, st, a);
-    if ((e = hipGetLastError()) != hipSuccess)
-        return e;
+        // Heads go round the XCDs first, splits last: sequences of unlike length leave the later
+        // splits empty, and with the splits first the XCDs that got those had nothing to do.
+        const dim3 grid((unsigned)a.c.n_kv, (unsigned)a.s.n_seq, (unsigned)(a.splits * a.tiles));
+        hipLaunchKernelGGL((k_kv4_attn<FMT, NG, T>), grid, dim3(256), 0, st, a);
+        if ((e = hipGetLastError()) != hipSuccess)
+            return e;
     }
     if (a.logit && !a.waves) {
         const int pairs = a.c.n_kv * a.s.n_seq;

@@ -146,24 +146,31 @@ hipError_t launch_qk_norm_rope(int dtype, int n_tok, int D, bool interleaved, Ro
 
 // ---- append and read-back -----------------------------------------------------------------
 
-// The sequence of row `tok`, and the row's token in it (may be negative: none).  A wave
-// counts the sequences that end at or before the row, 64 at a time; q_start does not fall.
+// The sequence of row `tok`, and the row's token in it (may be negative: none): the first that
+// ends behind the row (q_start does not fall).  A wave looks at 64 ends at a time, of more
+// sequences first at every 64th, so 16 and 4096 sequences take one and two round trips.
 // False for rows behind the last sequence (or ahead of the first).
 __device__ __forceinline__ bool kv4_find(const Kv4Seqs &s, int tok, int &seq, int &at, int &len) {
     const int lane = threadIdx.x & 63;
-    for (int b0 = 0; b0 < s.n_seq; b0 += 64) {
-        const int b = min(b0 + lane, s.n_seq - 1);
-        const int end = s.q_start[b + 1], n = s.lens[b];
-        const uint64_t later = __ballot(b0 + lane < s.n_seq && end > tok);
-        if (later) {
-            const int i = __builtin_ctzll(later);
-            seq = b0 + i;
-            len = __builtin_amdgcn_readlane(n, i);
-            at = len - __builtin_amdgcn_readlane(end, i) + tok;
-            return seq > 0 || tok >= s.q_start[0];
-        }
+    int b0 = 0, b1 = s.n_seq;
+    while (b1 - b0 > 64) {
+        const int step = (b1 - b0 + 63) / 64;
+        const uint64_t later = __ballot(s.q_start[min(b0 + (lane + 1) * step, b1)] > tok);
+        if (!later)
+            return false;
+        b0 += (int)__builtin_ctzll(later) * step;
+        b1 = min(b1, b0 + step);
     }
-    return false;
+    const int b = min(b0 + lane, b1 - 1);
+    const int end = s.q_start[b + 1], n = s.lens[b];
+    const uint64_t later = __ballot(b0 + lane < b1 && end > tok);
+    if (!later)
+        return false;
+    const int i = __builtin_ctzll(later);
+    seq = b0 + i;
+    len = __builtin_amdgcn_readlane(n, i);
+    at = len - __builtin_amdgcn_readlane(end, i) + tok;
+    return seq > 0 || tok >= s.q_start[0];
 }
 
 // Round to nearest, ties to even, of the real quotient x / s (s >= 2^-103): the product with

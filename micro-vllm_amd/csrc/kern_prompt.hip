@@ -35,6 +35,7 @@ __device__ __forceinline__ f4v mfma16(h8 a, h8 b, f4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 __device__ __forceinline__ h2 as_h2(uint32_t u) { return __builtin_bit_cast(h2, u); }
+__device__ __forceinline__ uint32_t as_u32(h2 h) { return __builtin_bit_cast(uint32_t, h); }
 __device__ __forceinline__ h2 round2(float a, float b) {
     return __builtin_convertvector(fl2{a, b}, h2);
 }
@@ -49,7 +50,8 @@ __device__ __forceinline__ float col_sum(float x) {
 // Largest of the wave's values, each not negative (ordered as their bits).
 __device__ __forceinline__ float wave_top(float x) {
     uint32_t v = __float_as_uint(x);
-#define TOP_STEP(ctrl) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, false))
+#define TOP_STEP(ctrl) \
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, false))
     TOP_STEP(0x111);  // row_shr:1, 2, 4, 8, then the rows' last lanes on to the next rows
     TOP_STEP(0x112);
     TOP_STEP(0x114);
@@ -59,7 +61,9 @@ __device__ __forceinline__ float wave_top(float x) {
 #undef TOP_STEP
     return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)v, 63));
 }
-__device__ __forceinline__ int exponent(float x) { return (int)((__float_as_uint(x) >> 23) & 255u) - 127; }
+__device__ __forceinline__ int exponent(float x) {
+    return (int)((__float_as_uint(x) >> 23) & 255u) - 127;
+}
 
 // What the scale wave says of a tile.
 struct TileInfo {
@@ -253,11 +257,12 @@ template <int FMT, int NG, typename T, int W, bool LSE> struct Prompt {
                         for (int j = 0; j < 4; ++j)
                             scaled(z[j], (float)s0, (float)s1, y[j]);
                     } else {
+                        // (the token's own pair of bytes, its own scale)
                         const uint32_t c[4] = {
-                            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, (float)s0, 0)),
-                            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, (float)s0, 1)),
-                            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, (float)s1, 2)),
-                            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, (float)s1, 3))};
+                            as_u32(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, (float)s0, 0)),
+                            as_u32(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, (float)s0, 1)),
+                            as_u32(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, (float)s1, 2)),
+                            as_u32(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, (float)s1, 3))};
                         y[0][0] = as_h2(__builtin_amdgcn_perm(c[2], c[0], 0x05040100u));
                         y[1][0] = as_h2(__builtin_amdgcn_perm(c[2], c[0], 0x07060302u));
                         y[2][0] = as_h2(__builtin_amdgcn_perm(c[3], c[1], 0x05040100u));
@@ -367,9 +372,10 @@ __global__ __launch_bounds__(64 * W, NG <= 2 ? 2 : 1) void k_kv4_prompt(AttnArgs
     for (int base = blockIdx.z / A.splits * 32 * W; base < rows; base += A.tiles * 32 * W) {
         const int last = min(rows, base + 32 * W) - 1;
         const int hi = max(0, min(pos0 + last / A.group + 1, len));
-        const int lo = A.window > 0 ? max(0, min(pos0 + base / A.group - A.window + 1, hi)) : 0;
-        const int s0 = (lo & ~(KT - 1)) + split * A.chunk;
-        const int s1 = split + 1 == A.splits ? hi : min(hi, s0 + A.chunk);
+        const int lo =
+            A.window > 0 ? max(0, min(max(pos0 + base / A.group, 0) - A.window + 1, hi)) : 0;
+        const int s0 = (int)min((long long)hi, (lo & ~(KT - 1)) + (long long)split * A.chunk);
+        const int s1 = split + 1 == A.splits ? hi : min(hi - s0, A.chunk) + s0;
         const int n_tiles = s1 > s0 ? (s1 - s0 + KT - 1) / KT : 0;
         Prompt<FMT, NG, T, W, LSE> P{A, L, A.s.table + (size_t)seq * A.s.max_pages, head, s0, s1, wave};
 
@@ -517,7 +523,9 @@ __global__ __launch_bounds__(64 * W, NG <= 2 ? 2 : 1) void k_kv4_prompt(AttnArgs
                 for (int c = 0; c < 2; ++c) {
                     // never 0: a masked -inf stays -inf
                     const float k2 = fmaxf(ldexpf(c2[c], I.ek + eq[c]), 0x1p-126f);
-                    const float k2lo = S::F32 ? ldexpf(fabsf(A.scale2) == A.scale2 ? A.scale2_lo : -A.scale2_lo, I.ek + eq[c]) : 0.f;
+                    const float k2lo =
+                        S::F32 ? ldexpf(A.scale2 < 0.f ? -A.scale2_lo : A.scale2_lo, I.ek + eq[c])
+                               : 0.f;
                     float top = -INFINITY;
 #pragma unroll
                     for (int b = 0; b < KT / 16; ++b) {

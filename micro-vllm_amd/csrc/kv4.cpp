@@ -1,5 +1,5 @@
 // kv4.cpp -- C entry points of attention over 4-bit keys and values: argument checks and
-// launches (the kernels are in kern_kv4.hip and kern_attn.hip).  The calls share no scratch
+// launches (the kernels are in kern_kv4.hip, kern_attn.hip and kern_prompt.hip).  The calls share no scratch
 // and keep no state: every buffer is the caller's.
 #include "../../include/mvllm_hip.h"
 
@@ -98,14 +98,17 @@ bool table_ok(const mvllm_kv4 *c, int max_pages) {
     return max_pages >= 1 && (long long)max_pages * c->page <= (1ll << 30);
 }
 
+// (a launch has fewer than 2^32 threads along a side: a workgroup a token)
+bool tokens_ok(int n_tok) { return n_tok >= 1 && n_tok <= (1 << 23); }
+
 const char *const kSeqRule =
-    ": bad sequences (q_start, lens and table, 1 <= n_seq <= 65535, n_tok >= 1, max_pages >= 1, "
-    "max_pages * page <= 2^30)";
+    ": bad sequences (q_start, lens and table, 1 <= n_seq <= 65535, 1 <= n_tok <= 2^23, max_pages "
+    ">= 1, max_pages * page <= 2^30, n_tok * n_kv * head_dim <= 2^34)";
 
 bool seqs_of(const mvllm_kv4 *c, int n_tok, const int *q_start, const int *lens, const int *table,
              int n_seq, int max_pages, Kv4Seqs &s) {
-    if (!q_start || !lens || !table || n_tok < 1 || n_seq < 1 || n_seq > 65535 ||
-        !table_ok(c, max_pages))
+    if (!q_start || !lens || !table || !tokens_ok(n_tok) || n_seq < 1 || n_seq > 65535 ||
+        !table_ok(c, max_pages) || (long long)n_tok * c->n_kv * c->head_dim > (1ll << 34))
         return false;
     s = Kv4Seqs{q_start, lens, table, n_seq, max_pages, n_tok};
     return true;
@@ -113,7 +116,8 @@ bool seqs_of(const mvllm_kv4 *c, int n_tok, const int *q_start, const int *lens,
 
 // A row of heads of `dtype`: 16-byte aligned, every `stride` elements.
 bool rows_ok(const void *p, long long stride, int dtype) {
-    return p && aligned16(p) && stride >= 0 && stride % (dtype == KV4_BF16 ? 8 : 4) == 0;
+    return p && aligned16(p) && stride >= 0 && stride <= (1ll << 36) &&
+           stride % (dtype == KV4_BF16 ? 8 : 4) == 0;
 }
 
 bool dtype_ok(int dtype) { return dtype == KV4_F32 || dtype == KV4_BF16; }
@@ -150,7 +154,7 @@ int mvllm_hip_qk_norm_rope_dev(int dtype, int n_tok, int head_dim, const void *q
                                const int *pos, const double *freq, int rot, int interleaved,
                                void *stream) {
     set_error("");
-    if (!dtype_ok(dtype) || n_tok < 1 || !head_dim_ok(head_dim) || n_q < 0 || n_kv < 0 ||
+    if (!dtype_ok(dtype) || !tokens_ok(n_tok) || !head_dim_ok(head_dim) || n_q < 0 || n_kv < 0 ||
         n_q + (long long)n_kv < 1 || n_q + (long long)n_kv > 65535 ||
         (n_q && (!rows_ok(q, q_stride, dtype) || !rows_ok(qo, qo_stride, dtype) ||
                  (n_tok > 1 && qo_stride < (long long)n_q * head_dim))) ||
@@ -158,8 +162,8 @@ int mvllm_hip_qk_norm_rope_dev(int dtype, int n_tok, int head_dim, const void *q
                   (n_tok > 1 && ko_stride < (long long)n_kv * head_dim))) ||
         !aligned16(wq) || !aligned16(wk) || !(eps >= 0.f) ||
         (freq && (!pos || rot < 16 || rot > head_dim || rot % 16)))
-        return refuse("qk_norm_rope_dev: bad arguments (dtype 0 or 1, n_tok >= 1, head_dim 64, "
-                      "128, 192 or 256, 1 <= n_q + n_kv <= 65535, 16-byte aligned rows and "
+        return refuse("qk_norm_rope_dev: bad arguments (dtype 0 or 1, 1 <= n_tok <= 2^23, head_dim "
+                      "64, 128, 192 or 256, 1 <= n_q + n_kv <= 65535, 16-byte aligned rows and "
                       "weights, output rows apart, eps >= 0, with freq: pos and rot a multiple of "
                       "16 up to head_dim)");
     RopeArgs a{};
@@ -213,8 +217,8 @@ int mvllm_hip_kv4_read_dev(const mvllm_kv4 *cache, int dtype, void *k, void *v, 
         return refuse(std::string("kv4_read_dev") + kCacheRule);
     if (!seqs_of(cache, n_tok, q_start, lens, table, n_seq, max_pages, s))
         return refuse(std::string("kv4_read_dev") + kSeqRule);
-    const size_t bytes =
-        rows_bytes(dtype, n_tok, (long long)c.n_kv * cache->head_dim, (long long)c.n_kv * cache->head_dim);
+    const long long row = (long long)c.n_kv * cache->head_dim;
+    const size_t bytes = rows_bytes(dtype, n_tok, row, row);
     if (!dtype_ok(dtype) || !k || !v || !aligned16(k) || !aligned16(v) ||
         ranges_meet(k, bytes, v, bytes))
         return refuse("kv4_read_dev: bad arguments (dtype 0 or 1, 16-byte aligned k and v that do "
@@ -227,8 +231,9 @@ int mvllm_hip_kv4_read_dev(const mvllm_kv4 *cache, int dtype, void *k, void *v, 
 static bool attention_sizes_ok(int head_dim, int n_kv, int n_q, int n_tok, int n_seq, int max_new,
                                int max_len) {
     return head_dim_ok(head_dim) && n_kv >= 1 && n_kv <= 1024 && n_q >= n_kv && n_q % n_kv == 0 &&
-           n_q <= 65535 && n_q / n_kv <= 1024 && n_tok >= 1 && n_seq >= 1 && n_seq <= 65535 && max_new >= 1 &&
-           max_len >= 1 && max_len <= (1 << 30) && (long long)n_tok * n_q <= (1ll << 30) &&
+           n_q <= 65535 && n_q / n_kv <= 1024 && tokens_ok(n_tok) && n_seq >= 1 &&
+           n_seq <= 65535 && max_new >= 1 && max_len >= 1 && max_len <= (1 << 30) &&
+           (long long)n_tok * n_q <= (1ll << 30) &&
            (long long)max_new * n_q <= (1ll << 30);
 }
 
@@ -257,17 +262,17 @@ int mvllm_hip_kv4_attention_dev(const mvllm_kv4 *cache, int dtype, const void *q
         !std::isfinite(scale) || window < 0 ||
         ranges_meet(q, rows_bytes(dtype, n_tok, q_stride, (long long)n_q * D), out,
                     rows_bytes(dtype, n_tok, (long long)n_q * D, (long long)n_q * D)))
-        return refuse("kv4_attention_dev: bad arguments (dtype 0 or 1, n_q a multiple of n_kv up to 1024 times it, "
-                      "16-byte aligned q and out that do not overlap, max_new >= 1, 1 <= max_len "
-                      "<= 2^30, n_tok * n_q and max_new * n_q up to 2^30, finite scale, window >= "
-                      "0)");
+        return refuse("kv4_attention_dev: bad arguments (dtype 0 or 1, n_q a multiple of n_kv up "
+                      "to 1024 times it, 16-byte aligned q and out that do not overlap, max_new "
+                      ">= 1, 1 <= max_len <= 2^30, n_tok * n_q and max_new * n_q up to 2^30, "
+                      "finite scale, window >= 0)");
     if (weights < KV4_WEIGHTS_NONE || weights > KV4_WEIGHTS_STORE ||
         (weights != KV4_WEIGHTS_NONE && !cache->score))
         return refuse("kv4_attention_dev: weights is 0, 1 or 2, and the cache has a score array "
                       "where it is not 0");
-    const AttnPlan p = kv4_attention_plan(kv4_rows_option(), cache->fmt, dtype, D, a.c.n_kv, n_q, n_tok, n_seq,
-                                          max_new, max_len, window,
-                                          weights != KV4_WEIGHTS_NONE);
+    const AttnPlan p =
+        kv4_attention_plan(kv4_rows_option(), cache->fmt, dtype, D, a.c.n_kv, n_q, n_tok, n_seq,
+                           max_new, max_len, window, weights != KV4_WEIGHTS_NONE);
     const size_t need = kv4_attention_bytes(D, a.c.n_kv, n_q, n_tok, n_seq, max_new, max_len,
                                             weights != KV4_WEIGHTS_NONE);
     if (need > work_bytes || (need && (!work || !aligned16(work))))
@@ -309,15 +314,16 @@ int mvllm_hip_kv4_evict_dev(const mvllm_kv4 *cache, const int *lens, const int *
     if (!view_of(cache, a.c) || !cache->score)
         return refuse(std::string("kv4_evict_dev") + kCacheRule + ", and a score array");
     if (!lens || !table || n_seq < 1 || n_seq > 65535 || !table_ok(cache, max_pages) ||
-        max_len < 1 || keep < 1 || recent < 0 || recent > keep || !dst_table ||
+        max_len < 1 || keep < 1 || keep > (1 << 29) || recent < 0 || recent > keep || !dst_table ||
         !table_ok(cache, dst_max_pages) || (long long)dst_max_pages * cache->page < keep ||
         !kept || !new_lens ||
         ranges_meet(table, (size_t)n_seq * max_pages * 4, dst_table,
                     (size_t)n_seq * dst_max_pages * 4) ||
         ranges_meet(lens, (size_t)n_seq * 4, new_lens, (size_t)n_seq * 4))
         return refuse("kv4_evict_dev: bad arguments (lens, table, 1 <= n_seq <= 65535, max_pages * "
-                      "page <= 2^30, max_len >= 1, 0 <= recent <= keep, keep >= 1, a dst_table of "
-                      "its own whose pages hold keep tokens, kept, and new_lens apart from lens)");
+                      "page <= 2^30, max_len >= 1, 0 <= recent <= keep, 1 <= keep <= 2^29, a "
+                      "dst_table of its own whose pages hold keep tokens, kept, and new_lens "
+                      "apart from lens)");
     a.lens = lens;
     a.table = table;
     a.dst_table = dst_table;

@@ -25,6 +25,10 @@ Bars, by the roundings that can meet (u = 2^-24, half an f32 step; h = 2^-8, hal
   denominator's share; f16 values and probabilities 3 f.
 - eviction: indices, codes, scales and scores equal.
 """
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -179,6 +183,35 @@ def test_append_and_read(hip, fmt, dtype, n_kv, D, page, lens, news):
                     if at else np.zeros((n_kv, D))
                 y = torch.from_numpy(y).float().to(TYPES[out_type])
                 assert torch.equal(got[r].cpu(), y)
+
+
+@pytest.mark.parametrize("n_seq", [64, 65, 129, 5000])
+def test_append_finds_its_sequence(hip, n_seq):
+    """Many sequences, some with no new token, several or fewer tokens than rows; rows ahead of
+    the first sequence and behind the last."""
+    rng = np.random.default_rng(n_seq)
+    news = rng.integers(0, 4, n_seq)
+    news[[0, n_seq // 2, n_seq - 1]] = 0, 3, 1
+    lens = news + rng.integers(-1, 3, n_seq).clip(-news)
+    qs = (starts(news) + 2).astype(np.int32)
+    T = int(qs[-1]) + 3
+    c = make_cache(rng, 7, 1, 64, 16, n_seq)
+    arr, cache = to_device(hip, c)
+    tab = rng.permutation(n_seq).reshape(-1, 1).astype(np.int32)
+    x = rng.standard_normal((2, T, 1, 64)).astype(np.float32)
+    xd = dev(x)
+    args = (T, dev(qs), dev(lens.astype(np.int32)), dev(tab), n_seq, 1)
+    hip.kv4_append_dev(cache, hip.F32, xd[0], 64, xd[1], 64, *args)
+    torch.cuda.synchronize()
+    codes, scales = kvref.quantize(7, x)
+    exp = {n: c[n].copy() for n in ("k", "ks", "v", "vs")}
+    for r, b, t in kvref.rows_of(qs, lens):
+        if t >= 0:
+            for i, n in enumerate("kv"):
+                exp[n][tab[b, 0], 0, t] = codes[i, r, 0]
+                exp[n + "s"][tab[b, 0], 0, t] = scales[i, r, 0]
+    for n in exp:
+        assert np.array_equal(host(arr[n]), exp[n]), n
 
 
 @pytest.mark.parametrize("fmt", [4, 7])
@@ -400,6 +433,22 @@ def test_attention_sizes_are_hints(hip, rows_kernel, max_new, max_len):
                         2)
     check_attention(c, host(q), host(out), host(arr["score"]), qs, ln, tab, 0.1, 0, 2, "f32",
                     forced=rows_kernel == 2)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_widest_window_and_rows_before_the_first_token(hip, rows_kernel, dtype):
+    """More rows than tokens under the widest window a call takes: the rows ahead of the first
+    token give zeros, and their positions take nothing from the rows they share a tile with."""
+    rng = np.random.default_rng(11)
+    c = make_cache(rng, 4, 2, 64, 32, 20)
+    lens, news = [7, 90], [20, 33]
+    tab, qs, ln = tables(rng, lens, 32, 20), starts(news), np.array(lens, np.int32)
+    arr, cache = to_device(hip, c)
+    q = torch.from_numpy(rng.standard_normal((53, 4, 64)).astype(np.float32)).cuda().to(TYPES[dtype])
+    out = run_attention(hip, cache, dtype, q, dev(qs), dev(ln), dev(tab), 33, 90, 0.2, 2 ** 31 - 1, 2)
+    check_attention(c, host(q), host(out), host(arr["score"]), qs, ln, tab, 0.2, 2 ** 31 - 1, 2, dtype,
+                    forced=rows_kernel == 2)
+    assert (host(out)[:13] == 0).all() and (host(out)[13:20] != 0).any()
 
 
 def test_attention_scales(hip, rows_kernel):
@@ -715,3 +764,39 @@ def test_stream_of_torch_and_null(hip):
                          None, None, 0)
     torch.cuda.synchronize()
     assert torch.equal(y, z)  # a power of two does not change the norm's roundings
+
+
+FIRST = """
+import numpy as np, torch
+import mvllm_hip as h
+h.init(0)
+h.set_option("kv4_rows", 2)
+z = lambda *s, dtype=torch.uint8: torch.zeros(s, dtype=dtype, device="cuda")
+i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")
+c = h.KV4(4, 1, 64, 32, z(8, 1, 32, 32), z(8, 1, 32, 1, dtype=torch.float32), z(8, 1, 32, 32),
+          z(8, 1, 32, 1, dtype=torch.float32), z(8, 1, 32, dtype=torch.float32))
+q, out = torch.ones(40, 1, 64, device="cuda"), torch.ones(40, 1, 64, device="cuda")
+kept, new, work = i32(*[7] * 16), i32(7), z(1 << 20)
+qs, ln, tab, dst = i32(0, 40), i32(100), i32(0, 1, 2, 3), i32(4)
+st = torch.cuda.Stream()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=st):
+    h.kv4_attention_dev(c, h.F32, q, 64, 1, 40, qs, ln, tab, 1, 4, 40, 100, 1.0, 0, 2, out, work,
+                        1 << 20, st)
+    h.kv4_evict_dev(c, ln, tab, 1, 4, 100, 16, 4, dst, 1, kept, new, st)
+for i in range(3):
+    out.fill_(1)
+    kept.fill_(7)
+    g.replay()
+    torch.cuda.synchronize()
+    assert (out == 0).all() and int(new) == 16 and kept.tolist() == [*range(12), *range(96, 100)], kept
+print("replayed")
+"""
+
+
+def test_first_call_of_a_process_is_captured():
+    """The calls that set a kernel up on their first use may make it inside a capture."""
+    p = subprocess.run([sys.executable, "-c", FIRST], capture_output=True, text=True, timeout=100,
+                       env=os.environ | {"PYTHONPATH": os.pathsep.join(sys.path)})
+    assert p.returncode == 0 and "replayed" in p.stdout, p.stderr[-2000:]

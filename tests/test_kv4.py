@@ -134,6 +134,28 @@ def test_evict_refuses():
         call(cache(score=None))
 
 
+@pytest.mark.parametrize("n_kv,D,n_tok", [(1, 64, (1 << 23) + 1), (1024, 256, (1 << 16) + 1)])
+def test_launches_past_32_bits_are_refused(n_kv, D, n_tok):
+    """More tokens than a launch has threads for."""
+    c, big = cache(n_kv=n_kv, head_dim=D), 1 << 50
+    s = (n_tok, A, A, A, 2, 4)
+    refused("bad sequences", mvllm_hip.kv4_append_dev, c, BF16, A, 0, A, 0, *s)
+    refused("bad sequences", mvllm_hip.kv4_read_dev, c, BF16, A, big, *s)
+    refused("bad sequences", mvllm_hip.kv4_attention_dev, c, BF16, A, 0, n_kv, *s, 1, 100, 0.1, 0, 0,
+            big, A, 1 << 50)
+
+
+def test_large_sizes_are_refused():
+    c = cache()
+    refused("bad arguments", mvllm_hip.qk_norm_rope_dev, F32, (1 << 23) + 1, 64, A, 64, 1, A, 64, None,
+            0, 0, None, 0, None, None, 0.0, None, None, 0)
+    refused("bad arguments", mvllm_hip.kv4_append_dev, c, F32, A, 1 << 40, A, 512, 4, A, A, A, 2, 4)
+    refused("bad arguments", mvllm_hip.kv4_evict_dev, c, A, A, 2, 4, 200, (1 << 29) + 1, 8, 2 * A,
+            1 << 24, A, 3 * A)
+    with pytest.raises(HipError):
+        mvllm_hip.kv4_attention_work(1, 64, 1, (1 << 23) + 1, 1, 1, 100)
+
+
 def test_rope_refuses():
     ok = dict(dtype=F32, T=3, D=128, q=A, qs=1024, nq=8, qo=2 * A, qos=1024, k=A, ks=1024, nk=2,
               ko=3 * A, kos=256, wq=A, wk=A, eps=1e-6, pos=A, freq=A, rot=64)
