@@ -111,9 +111,11 @@ __device__ __forceinline__ void span_of(const AttnArgs &A, const Tile &t, int r0
 }
 
 // B operands of 16 rows of queries: lane (column c, group of lanes kg) holds, of each 64
-// elements g, the 16 from 64 g + 16 kg, as two operands (int4: in decode_b<4>'s order).  k8: -8
-// times a row's sum of queries in each group, from which the sums of products with int4 codes n
-// start, so that they end as those with n - 8 (one instruction for 4 codes in place of five).
+// elements g, the 16 from 64 g + 16 kg, as two operands (int4: in decode_b<4>'s order).  k8, of
+// bf16 queries: -8 times a row's sum of queries in each group, from which the sums of products
+// with int4 codes n start, so that they end as those with n - 8 (one instruction for 4 codes in
+// place of five).  f32 calls take n - 8 itself: the larger sums on the way make their
+// outputs' error 1.1e-6 in place of 4e-7 (16 streams to 4096 tokens; 43.8 and 44.7 us).
 template <int FMT, int NG, int TQ, typename T>
 __device__ __forceinline__ void load_q(const AttnArgs &A, const Tile &t, int row, bool live,
                                        bf16x8 (&q)[NG][2][TQ], float (&k8)[NG]) {
@@ -136,7 +138,7 @@ __device__ __forceinline__ void load_q(const AttnArgs &A, const Tile &t, int row
                 y[a_slot<FMT>(e)] = x[e];
             split8<TQ>(y, q[g][s]);
         }
-        k8[g] = FMT == 4 ? -8.f * col_sum(sum) : 0.f;
+        k8[g] = FMT == 4 && TQ == 1 ? -8.f * col_sum(sum) : 0.f;
     }
 }
 
@@ -177,8 +179,9 @@ __device__ __forceinline__ f4v dot_keys(const Keys<FMT, NG> &k, const bf16x8 (&q
     f4v sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-        const bf16x8 a0 = decode_b<FMT>(k.w[g].x, FMT == 7 ? k.s[g] : 0.f);
-        const bf16x8 a1 = decode_b<FMT>(k.w[g].y, FMT == 7 ? k.s[g] : 0.f);
+        const float s7 = FMT == 7 ? k.s[g] : 0.f;
+        const bf16x8 a0 = FMT == 4 && TQ > 1 ? decode_b4_signed(k.w[g].x) : decode_b<FMT>(k.w[g].x, s7);
+        const bf16x8 a1 = FMT == 4 && TQ > 1 ? decode_b4_signed(k.w[g].y) : decode_b<FMT>(k.w[g].y, s7);
         f4v acc = FMT == 4 ? f4v{k8[g], k8[g], k8[g], k8[g]} : sum;
 #pragma unroll
         for (int t = TQ - 1; t >= 0; --t) {
