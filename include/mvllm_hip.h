@@ -356,9 +356,9 @@ int mvllm_hip_kv4_read_dev(const mvllm_kv4 *cache, int dtype, void *k, void *v, 
  * that are short: the codes enter the bf16 matrix cores exactly; f32 queries and probabilities
  * as three bf16 terms (all 24 bits), bf16 queries exactly and their probabilities as two terms.
  * Long calls of more rows run on f16 operands with powers of two taken out: bf16 calls round
- * probabilities, and int4 codes times their scales, once by 2^-12; f32 calls hold such operands in
- * two terms (2^-23), and so do the exponents of calls that collect weights.  Sums, maxima and
- * exponentials are f32.
+ * probabilities, int4 codes times their scales and int4 values' scales by up to 2^-11 each; f32
+ * calls hold such operands in two terms (2^-22), and so do the exponents of calls that collect
+ * weights.  Sums, maxima and exponentials are f32.
  * weights: 1 adds to score, 2 stores into it, for each of the sequences' tokens, the sum of its
  * P over the call's new tokens and the kv head's group of query heads (0 where none sees it).
  * Sequences that share pages may attend together with weights 0; their scores would be two

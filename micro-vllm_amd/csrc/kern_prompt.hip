@@ -10,10 +10,13 @@
 // tile of keys by its largest scale, the values by the largest scale so far (the sums move
 // along), so that each set's largest magnitude lies near 2^14 and what is up to 2^28 smaller
 // keeps its 11 bits.  bf16 queries and MXFP4 codes times their scales are then exact; int4 codes
-// times their scales, and probabilities, are rounded by 2^-12 of themselves (bf16 outputs round
-// by 2^-8; bf16 operands would have added as much again).  f32 calls take two f16 terms of
-// each rounded operand and leave out the product of the two second ones (2^-23); calls that
-// collect weights two of the keys.
+// times their scales, and probabilities, are rounded by up to 2^-11 of themselves, values' scales
+// before as well (bf16 outputs round by 2^-8; bf16 operands would have added as much again).
+// Keys' scales are not: a token's exponents would all be off by its scale's rounding, which
+// 6000 tokens of narrow heads made half as much again as the output's own rounding (2-norm 2.4e-3
+// of it, 1.9e-3 so; 64-element heads).  f32 calls take two f16 terms of each rounded operand and
+// leave out the product of the two second ones (2^-22 each); calls that collect weights two
+// of the keys.
 //
 // A tile's scales are prepared by one wave, in turn, two tiles ahead: it takes the powers out,
 // zeroes the scales of tokens that are not there, and gives a token whose value scales are not
@@ -80,8 +83,9 @@ template <int FMT, int NG, typename T, bool LSE> struct PromptShape {
     static constexpr int QT = F32 ? 2 : 1;
     static constexpr int KKT = FMT == 4 && (F32 || LSE) ? 2 : 1, KVT = FMT == 4 && F32 ? 2 : 1;
     static constexpr int SB = FMT == 4 ? NG : 2 * NG;  // scales of a row
-    // a scale as the decoding reads it: f16 where the product is rounded to f16 anyway
-    using KScale = std::conditional_t<FMT == 4 && KKT == 1, _Float16, float>;
+    // a scale as the decoding reads it, where its product with a code is rounded to f16: of
+    // values an f16, of keys an f16 and what that leaves
+    using KScale = std::conditional_t<FMT == 4 && KKT == 1, h2, float>;
     using VScale = std::conditional_t<FMT == 4 && KVT == 1, _Float16, float>;
     struct Buf {
         h8 k[KKT][KT / 16][KS][64];
@@ -182,16 +186,18 @@ template <int FMT, int NG, typename T, int W, bool LSE> struct Prompt {
         }
     }
 
-    // (n - 8) * s as f16, or as two terms of the f32 product.
-    template <int N>
-    __device__ __forceinline__ static void scaled(h2 n, float s0, float s1, h2 (&o)[N]) {
-        if constexpr (N == 2) {
-            const float a = (float)n[0] * s0, b = (float)n[1] * s1;
-            o[0] = round2(a, b);
-            o[N - 1] = round2(a - (float)o[0][0], b - (float)o[0][1]);
-        } else {
-            o[0] = n * h2{(_Float16)s0, (_Float16)s1};
-        }
+    // (n - 8) * s, rounded to f16: keys' with one rounding, values' with the scale's own before.
+    __device__ __forceinline__ static void scaled(h2 n, h2 s, h2, h2 (&o)[1]) {
+        o[0] = __builtin_elementwise_fma(n, h2{s[0], s[0]}, n * h2{s[1], s[1]});
+    }
+    __device__ __forceinline__ static void scaled(h2 n, _Float16 s0, _Float16 s1, h2 (&o)[1]) {
+        o[0] = n * h2{s0, s1};
+    }
+    // Two terms of the f32 product.
+    __device__ __forceinline__ static void scaled(h2 n, float s0, float s1, h2 (&o)[2]) {
+        const float a = (float)n[0] * s0, b = (float)n[1] * s1;
+        o[0] = round2(a, b);
+        o[1] = round2(a - (float)o[0][0], b - (float)o[0][1]);
     }
 
     // Decodes the fetched tile into its buffer.
@@ -215,7 +221,7 @@ template <int FMT, int NG, typename T, int W, bool LSE> struct Prompt {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             h2 y[KKT];
-                            scaled(x[e], (float)s, (float)s, y);
+                            scaled(x[e], s, s, y);
 #pragma unroll
                             for (int k = 0; k < KKT; ++k) {
                                 o[k][2 * e] = y[k][0];
@@ -224,10 +230,10 @@ template <int FMT, int NG, typename T, int W, bool LSE> struct Prompt {
                         }
                     } else {
                         const h2 x[4] = {
-                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word[j], (float)s, 0),
-                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word[j], (float)s, 1),
-                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word[j], (float)s, 2),
-                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word[j], (float)s, 3)};
+                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word[j], s, 0),
+                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word[j], s, 1),
+                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word[j], s, 2),
+                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word[j], s, 3)};
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             o[0][2 * e] = x[e][0];
@@ -255,14 +261,14 @@ template <int FMT, int NG, typename T, int W, bool LSE> struct Prompt {
                         int4_pairs(x >> 8, z[2], z[3]);
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            scaled(z[j], (float)s0, (float)s1, y[j]);
+                            scaled(z[j], s0, s1, y[j]);
                     } else {
                         // (the token's own pair of bytes, its own scale)
                         const uint32_t c[4] = {
-                            as_u32(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, (float)s0, 0)),
-                            as_u32(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, (float)s0, 1)),
-                            as_u32(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, (float)s1, 2)),
-                            as_u32(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, (float)s1, 3))};
+                            as_u32(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, s0, 0)),
+                            as_u32(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, s0, 1)),
+                            as_u32(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, s1, 2)),
+                            as_u32(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, s1, 3))};
                         y[0][0] = as_h2(__builtin_amdgcn_perm(c[2], c[0], 0x05040100u));
                         y[1][0] = as_h2(__builtin_amdgcn_perm(c[2], c[0], 0x07060302u));
                         y[2][0] = as_h2(__builtin_amdgcn_perm(c[3], c[1], 0x05040100u));
@@ -333,7 +339,10 @@ template <int FMT, int NG, typename T, int W, bool LSE> struct Prompt {
 #pragma unroll
             for (int g = 0; g < SB; ++g) {
                 const float k = there && !good ? NAN : ldexpf(sk[g], -ek);
-                L.sk[tile & 1][g][t] = (typename S::KScale)k;
+                if constexpr (std::is_same_v<typename S::KScale, h2>)
+                    L.sk[tile & 1][g][t] = h2{(_Float16)k, (_Float16)(k - (float)(_Float16)k)};
+                else
+                    L.sk[tile & 1][g][t] = k;
                 L.sv[tile & 1][g][t] = (typename S::VScale)ldexpf(sv[g], -max(ev, -400));
             }
         }

@@ -10,19 +10,18 @@ Bars, by the roundings that can meet (u = 2^-24, half an f32 step; h = 2^-8, hal
   of itself, a probability by ln 2 of that and 2 u, in numerator and denominator; the sums of n
   products add (n + 64) u of sum P |v|.  bf16: probabilities as two terms (h^2 / 2 of sum P |v|)
   and the output's own h.
-- attention of more than 16 rows of a kv head (maybe f16 operands, f = 2^-12 half an f16 step): bf16
-  calls round a probability once (f), an int4 scale and its product with a code once each, of
-  keys (an exponent is off by 2 f of sum |q k|) and of values (2 f of sum P |v|); MXFP4 is exact.
-  f32 calls hold each rounded operand in two terms (f^2 of it, 2^-24, taken as 2 u for its
-  subnormal second terms) and leave out the product of the second two (f^2): 3 * 2 u of sum
-  |q k| and of sum P |v|.  So do the exponents of calls that collect weights, whose own sums
-  take exact products.  Below 2^-14 an f16 holds steps of 2^-24: probabilities are carried so
-  that the largest is 2^7 (bf16; 2^14 f32) or more, so each of n is off by 2^-32 (2^-39) of
-  the row's sum at least, and a value by 2^-25 of 2^14 for the largest of its tile: n 2^-31
-  (2^-38) of the largest |v| beside the rest.
+- attention of more than 16 rows of a kv head (maybe f16 operands, f = 2^-11 half an f16 step, eps / 2):
+  bf16 calls round a probability (f), a key's int4 code times its scale (f: an exponent is off by
+  f of sum |q k|), a value's int4 scale and its product with a code (2 f of sum P |v|); MXFP4 is
+  exact.  f32 calls hold each rounded operand in two terms (f^2 = 4 u of it, twice a product)
+  and leave out the product of the second two (f^2): 12 u of sum |q k| and of sum P |v|.  So do
+  the exponents of calls that collect weights, whose own sums take exact products.  Below
+  2^-14 an f16 holds steps of 2^-24: probabilities are carried so that the largest is 2^7 (bf16;
+  2^14 f32) or more, so each of n is off by 2^-32 (2^-39) of the row's sum at least, and a value
+  by 2^-25 of 2^14 for the largest of its tile: n 2^-31 (2^-38) of the largest |v| beside the rest.
 - the 2-norm: errors of independent roundings grow as their root: exponents 4 u of the largest
-  one, 16 u beside; f16 keys' 2 f of the root of the sum of (q k)^2, twice for the
-  denominator's share; f16 values and probabilities 3 f.
+  one, 16 u beside; f16 keys' f of the root of the sum of (q k)^2, twice for the denominator's
+  share; f16 values and probabilities 3 f.
 - eviction: indices, codes, scales and scores equal.
 """
 import os
@@ -271,10 +270,10 @@ def check_attention(c, q, got, score, q_start, lens, tab, scale, window, weights
     own = ~np.isnan(out).all((1, 2))
     assert (got[~own] == fill).all()
     prompt = int(np.max(np.diff(q_start))) * (q.shape[1] // c["k"].shape[1]) > 16 or forced
-    f = 2.0 ** -12 if prompt else 0.0
-    k_off = (2 * f if c["fmt"] == 4 else 0) if dtype == "bf16" else 6 * U * prompt
-    v_off = (3 * f if c["fmt"] == 4 else f) if dtype == "bf16" else 6 * U * prompt
-    w_off = 6 * U * prompt
+    f = 2.0 ** -11 if prompt else 0.0
+    k_off = (f if c["fmt"] == 4 else 0) if dtype == "bf16" else 12 * U * prompt
+    v_off = (3 * f if c["fmt"] == 4 else f) if dtype == "bf16" else 12 * U * prompt
+    w_off = 12 * U * prompt
     if weights:
         k_off = w_off
     p_off = 2 * (np.log(2) * (U * (D * sums + 2 * top) + k_off * sums) + 2 * U)
@@ -668,7 +667,7 @@ def test_prompt_decode_evict_decode(hip, fmt, dtype):
             score[pl[0], :, pl[1]] = 0
         out, mag, (top, _, root), score = kvref.attention(now, host(st["q"]), qs, held, tab,
                                                           128 ** -0.5, 0, 1)
-        f, k_off = (2.0 ** -12, 6 * U) if st is p else (0.0, 0.0)  # many rows, maybe f16
+        f, k_off = (2.0 ** -11, 12 * U) if st is p else (0.0, 0.0)  # many rows, maybe f16
         tol = (4 * top + 16) * U + (H if dtype == "bf16" else 0) + 2 * k_off * root + 3 * f
         assert np.linalg.norm(host(st["out"]) - out) <= tol * np.linalg.norm(out)
         assert np.linalg.norm(host(st["arr"]["score"]) - score) <= \
