@@ -43,12 +43,15 @@ __device__ __forceinline__ float col_sum(float x) {
     return x + __shfl_xor(x, 32);
 }
 
-// 2^(s * scale * log2(e) - ref) in one rounding of the exponent; f32 inputs take the part of
+// s * scale * log2(e) - ref in one rounding, and its power of two; f32 inputs take the part of
 // scale * log2(e) that an f32 does not hold along (it would be off by 3e-8 of each exponent).
-template <typename T> __device__ __forceinline__ float power(const AttnArgs &A, float s, float ref) {
+template <typename T> __device__ __forceinline__ float exponent(const AttnArgs &A, float s, float ref) {
     if constexpr (sizeof(T) == 4)
-        return __builtin_amdgcn_exp2f(fmaf(s, A.scale2, fmaf(s, A.scale2_lo, -ref)));
-    return __builtin_amdgcn_exp2f(fmaf(s, A.scale2, -ref));
+        return fmaf(s, A.scale2, fmaf(s, A.scale2_lo, -ref));
+    return fmaf(s, A.scale2, -ref);
+}
+template <typename T> __device__ __forceinline__ float power(const AttnArgs &A, float s, float ref) {
+    return __builtin_amdgcn_exp2f(exponent<T>(A, s, ref));
 }
 
 // x[8] as T bf16 operands that add up to it (T = 3: all 24 bits).  An infinite x becomes NaN,
@@ -116,7 +119,11 @@ __device__ __forceinline__ void span_of(const AttnArgs &A, const Tile &t, int r0
 // with int4 codes n start, so that they end as those with n - 8 (one instruction for 4 codes in
 // place of five).  f32 calls take n - 8 itself: the larger sums on the way make their
 // outputs' error 1.1e-6 in place of 4e-7 (16 streams to 4096 tokens; 43.8 and 44.7 us).
-template <int FMT, int NG, int TQ, typename T>
+// Rows that are not live: zeros (GUARD), or the sequence's first one's queries (there is one).
+// Loads without a branch start sooner, which f32 rows gain by (16 streams to 4096 tokens 41.7 us,
+// 45.0 with it); half empty tiles of bf16 ones are better with it (32 streams to 16384 tokens,
+// groups of 8: 96.3 and 98.3).
+template <int FMT, int NG, int TQ, typename T, bool GUARD>
 __device__ __forceinline__ void load_q(const AttnArgs &A, const Tile &t, int row, bool live,
                                        bf16x8 (&q)[NG][2][TQ], float (&k8)[NG]) {
     const int kg = (threadIdx.x & 63) >> 4;
@@ -130,7 +137,7 @@ __device__ __forceinline__ void load_q(const AttnArgs &A, const Tile &t, int row
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, y[8];
-            if (live)
+            if (!GUARD || live)
                 Vec8<T>::load(p + 64 * g + 8 * s, x);
             sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
 #pragma unroll
@@ -557,7 +564,7 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
         }
         bf16x8 q[NG][2][TQ];
         float k8[NG];
-        load_q<FMT, NG, TQ, T>(A, t, row, live, q, k8);
+        load_q<FMT, NG, TQ, T, TQ == 1>(A, t, row, live, q, k8);
         typename V::Acc o;
         o.clear();
         float m = -INFINITY, l = 0.f;
@@ -873,9 +880,9 @@ __global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs A) {
         const int i = live ? token_of(A, row) : 0;
         pos = t.pos0 + i;
         from = A.window > 0 ? pos - A.window : -1;
-        lse = live ? A.lse[(size_t)(t.first + i) * A.n_q + t.head * A.group + row - i * A.group]
-                   : -INFINITY;
-        load_q<FMT, NG, TQ, T>(A, t, row, live, q, k8);
+        lse = A.lse[(size_t)(t.first + i) * A.n_q + t.head * A.group +
+                    (live ? row - i * A.group : 0)];
+        load_q<FMT, NG, TQ, T, false>(A, t, row, live, q, k8);
     };
     Keys<FMT, NG> k[NB], ahead[FEW ? NB : 1];
     bool ok[NB];
@@ -898,7 +905,7 @@ __global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs A) {
     if (FEW && t0 < len)
         fetch(t0, ahead);
     const bool once = FEW && t.rows <= 16;
-    if (once && t0 < len)
+    if (once && t0 < len && t.rows > 0)
         rows_at(0);
     for (; t0 < len; t0 += step) {
         bool there[NB];
@@ -921,20 +928,32 @@ __global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs A) {
             }
         }
         float w[NB][4] = {};
-        auto add = [&] {
+        // whole: every row sees every token
+        auto add = [&](bool whole) {
 #pragma unroll
             for (int h = 0; h < NB; ++h) {
                 const f4v s = dot_keys<FMT, NG, TQ>(k[h], q, k8);
+                float x[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int tok = t0 + 16 * h + 4 * kg + i;
-                    const bool sees = live && tok <= pos && tok > from;
-                    w[h][i] += sees ? power<T>(A, s[i], lse) : 0.f;
+                for (int i = 0; i < 4; ++i)
+                    x[i] = exponent<T>(A, s[i], lse);
+                if (!whole) {
+                    asm volatile("");  // a branch; within it selects, no branch an element
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int tok = t0 + 16 * h + 4 * kg + i;
+                        const bool sees = live & (tok <= pos) & (tok > from);
+                        x[i] = sees ? x[i] : -INFINITY;
+                    }
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    w[h][i] += __builtin_amdgcn_exp2f(x[i]);
             }
         };
         if (once) {
-            add();
+            if (t.rows > 0)
+                add(false);
         } else {
             // from the first row that may see the first token to the last whose window holds
             // the last one
@@ -945,7 +964,8 @@ __global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs A) {
                                 max(0ll, (long long)t0 + BLK - 1 + A.window - t.pos0) * A.group);
             for (r = (r & ~15) + (FEW ? 0 : 16 * wave); r < rend; r += FEW ? 16 : 64) {
                 rows_at(r);
-                add();
+                add(r + 16 <= t.rows && t0 + BLK - 1 <= t.pos0 + token_of(A, r) &&
+                    (A.window == 0 || t0 > t.pos0 + token_of(A, r + 15) - A.window));
             }
         }
         // a lane's four tokens of each 16, over the 16 rows of its columns; lane (kg, col < 4)
