@@ -741,6 +741,31 @@ __global__ __launch_bounds__(256) void k_kv4_join(AttnArgs A) {
     join<NG, T>(A, blockIdx.x, blockIdx.y * 4 + (threadIdx.x >> 6));
 }
 
+// One row's products with four tokens' keys from cache row `place` on, a key after the other.
+template <int FMT, int NG, typename T>
+__device__ __forceinline__ void dot_four(const AttnArgs &A, size_t place, const T *q, float (&s)[4]) {
+    constexpr int D = 64 * NG;
+#pragma unroll 1
+    for (int e = 0; e < 4; ++e) {
+        const size_t row = place + e;
+        float sum = 0.f;
+#pragma unroll 1
+        for (int d = 0; d < D; d += 8) {
+            const float sc = FMT == 4 ? reinterpret_cast<const float *>(A.c.ks)[row * NG + d / 64]
+                                      : ue8m0_ref(A.c.ks[row * (2 * NG) + d / 32]);
+            const uint32_t c = reinterpret_cast<const uint32_t *>(A.c.k)[(row * D + d) / 8];
+            float part = 0.f;
+#pragma unroll
+            for (int z = 0; z < 8; ++z) {
+                const uint32_t x = (c >> (4 * z)) & 15u;
+                part = fmaf((float)q[d + z], FMT == 4 ? (float)((int)x - 8) : e2m1_val(x), part);
+            }
+            sum = fmaf(part, sc, sum);
+        }
+        s[e] = sum;
+    }
+}
+
 // The end of a decode call that collects weights, in one launch.  The first `joins` workgroups
 // join the splits, as above.  The others take 1024 tokens each of one sequence and kv head, four
 // a thread: the rows' maxima and sums from the splits', the tokens' logits as the attention
@@ -802,48 +827,40 @@ __global__ __launch_bounds__(256) void k_kv4_finish(AttnArgs A, int joins) {
                 continue;
             const size_t place = kv4_row(A.c, phys, t.head, t0 - pg * A.c.page);
             float w[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int n = 0; n < n_rows; ++n) {
-                const int r = r0 + n, i = token_of(A, r), pos = t.pos0 + i;
-                const int head = t.head * A.group + r - i * A.group;
-                const int from = A.window > 0 ? pos - A.window : -1;
-                if (t0 > pos || t0 + 3 <= from)
-                    continue;
-                float s[4];
-                if (t0 < A.logits) {
-                    const float4 y = *reinterpret_cast<const float4 *>(
-                        A.logit + ((size_t)(t.first + i) * A.n_q + head) * (size_t)A.logits + t0);
-                    s[0] = y.x; s[1] = y.y; s[2] = y.z; s[3] = y.w;
-                } else {
-                    const T *q = static_cast<const T *>(A.q) + (size_t)(t.first + i) * A.q_stride +
-                                 (size_t)head * D;
-#pragma unroll 1
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t *k =
-                            reinterpret_cast<const uint32_t *>(A.c.k) + (place + e) * (D / 8);
-                        float sum = 0.f;
-#pragma unroll 1
-                        for (int d = 0; d < D; d += 8) {
-                            const float sc =
-                                FMT == 4 ? reinterpret_cast<const float *>(
-                                               A.c.ks)[(place + e) * NG + d / 64]
-                                         : ue8m0_ref(A.c.ks[(place + e) * (2 * NG) + d / 32]);
-                            const uint32_t c = k[d / 8];
-                            float part = 0.f;
+            const bool kept = t0 < A.logits;
+            for (int n0 = 0; n0 < n_rows; n0 += 4) {
+                float4 y[4] = {};  // four rows' logits on their way
+                if (kept) {
 #pragma unroll
-                            for (int z = 0; z < 8; ++z) {
-                                const uint32_t x = (c >> (4 * z)) & 15u;
-                                part = fmaf((float)q[d + z],
-                                            FMT == 4 ? (float)((int)x - 8) : e2m1_val(x), part);
-                            }
-                            sum = fmaf(part, sc, sum);
-                        }
-                        s[e] = sum;
+                    for (int u = 0; u < 4; ++u) {
+                        const int r = r0 + min(n0 + u, n_rows - 1), i = token_of(A, r);
+                        y[u] = *reinterpret_cast<const float4 *>(
+                            A.logit +
+                            ((size_t)(t.first + i) * A.n_q + t.head * A.group + r - i * A.group) *
+                                (size_t)A.logits +
+                            t0);
                     }
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (t0 + e <= pos && t0 + e > from)
-                        w[e] += power<T>(A, s[e], lse[n]);
+                for (int u = 0; u < 4; ++u) {
+                    const int n = n0 + u, r = r0 + n, i = token_of(A, r), pos = t.pos0 + i;
+                    const int from = A.window > 0 ? pos - A.window : -1;
+                    if (n >= n_rows)  // (of the whole workgroup)
+                        break;
+                    float s[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+                    if (!kept)
+                        dot_four<FMT, NG, T>(A, place,
+                                             static_cast<const T *>(A.q) +
+                                                 (size_t)(t.first + i) * A.q_stride +
+                                                 (size_t)(t.head * A.group + r - i * A.group) * D,
+                                             s);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool sees = (t0 + e <= pos) & (t0 + e > from);
+                        const float x = exponent<T>(A, s[e], lse[n]);
+                        w[e] += __builtin_amdgcn_exp2f(sees ? x : -INFINITY);
+                    }
+                }
             }
             float *p = A.c.score + place;
 #pragma unroll
