@@ -1024,12 +1024,16 @@ __global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs A) {
 // How a call is cut, for the 16-row kernel or (prompt) that of kern_prompt.hip, 8 waves of 32 rows
 // a workgroup (4 for head_dim 192 and 256, whose sums fill the registers).
 //
-// Splits of the tokens: enough workgroups to fill the chip (`fill`), but chunks of 128 tokens
-// (one block a wave) at least, and at most the 64 splits that a wave joins.  A workgroup's
-// start and end cost about as much as three blocks, so where registers allow two workgroups a
-// CU anyway, three times the CUs are best (768: 16 f32 int4 streams to 4096 tokens 54 us, 58 with
-// 2048, 62 with 512); bf16 over MXFP4, three a CU and less work a block, gains by finer chunks
-// (32 streams to 16384 tokens 110 us with 2048, 120 with 768).
+// Splits of the tokens, at most the 64 that a wave joins, in chunks of 128 tokens (one block a
+// wave) at least, 384 of long sequences (12 heads' rows over 11000 tokens: 29 splits 15.0 us, 43
+// 17.0); up to 384 tokens stay whole, which saves the join (300 tokens: 9.2 us, 11.2 in three).
+// The 16-row kernel: as many as make one round of
+// the chip with every sequence full, two workgroups a CU, or three of bf16 over MXFP4 (8 f32
+// MXFP4 streams of 8 kv heads, all of 8192 tokens: 8 splits 27 us, 7 and 10 35; of 1000 to 8192
+// 26, and 30 with 12).  Where its chunks are long, more, since lengths differ and the rounds even
+// out: chunks of 1408 tokens up to one and a half rounds (16 int4 f32 streams of 16 heads, 100
+// to 4096 tokens: 2 splits 50 us, 3 39, 4 47, 8 45; all of 4096: 55, 57, 57, 63), and of 2048 up
+// to four (32 MXFP4 bf16 streams of 8 heads, 4096 to 16384: 3 splits 105 us, 8 96, 16 106).
 static AttnPlan plan_for(bool prompt, int fmt, int dtype, int head_dim, int n_kv, int n_q,
                          int n_tok, int n_seq, int max_new, int max_len, int window,
                          bool weights) {
@@ -1037,14 +1041,20 @@ static AttnPlan plan_for(bool prompt, int fmt, int dtype, int head_dim, int n_kv
     const long long rows = (long long)max_new * (n_q / n_kv), pairs = (long long)n_kv * n_seq;
     p.waves = !prompt ? 0 : head_dim <= 128 ? 8 : 4;
     const int tile = p.waves ? 32 * p.waves : 16, least = p.waves ? 256 : 128;
-    const int fill = p.waves ? 256 : fmt == 7 && dtype == KV4_BF16 ? 2048 : 768;
+    const int slots = p.waves ? 256 : fmt == 7 && dtype == KV4_BF16 ? 768 : 512;
     p.tiles = (int)std::min(32768ll, (rows + tile - 1) / tile);
     // the most tokens that a tile's rows see, from a multiple of 64 on
     const long long seen =
         window > 0 ? std::min((long long)max_len, (long long)window + tile / (n_q / n_kv) + 65)
                    : max_len;
-    const long long want = std::max(1ll, std::min(64ll, fill / (p.tiles * pairs)));
-    p.chunk = (int)std::max((long long)least, ((seen + want - 1) / want + 127) / 128 * 128);
+    const long long each = p.tiles * pairs;  // workgroups of a split
+    long long want = slots / each;
+    if (!p.waves)
+        want = std::max({want, std::min(slots * 3 / 2 / each, (seen + 1407) / 1408),
+                         std::min(slots * 4 / each, (seen + 2047) / 2048)});
+    want = seen <= 384 ? 1 : std::max(1ll, std::min(64ll, want));
+    p.chunk = (int)std::max({(long long)least, ((seen + want - 1) / want + 127) / 128 * 128,
+                             p.waves ? 0 : std::min(384ll, (seen / 32 + 127) / 128 * 128)});
     p.splits = (int)((seen + p.chunk - 1) / p.chunk);
     auto add = [&](size_t bytes) {
         const size_t at = p.bytes;
