@@ -492,11 +492,19 @@ constexpr int attn_waves(int fmt, int ng, bool f32) {
 // free, and the value loads follow it.  Codes go from memory to the operands in registers.
 //
 // Each wave asks for the next block's keys as soon as it is done with this one's, so they are
-// on their way during the exponentials and the second product, and for its values after that:
-// what bounds the kernel is how many bytes are on their way.  (Two whole blocks in registers
-// halve the waves that fit.)  The pool pages are looked up one block earlier.  The maximum is
-// raised only when a block passes it by 2^8 (sums stay in range, and relative precision does
-// not depend on it), so most blocks need no exchange between lanes and no rescaling.
+// on their way during the exponentials and the second product, and for its values after that
+// (two whole blocks in registers gained nothing and halved the waves that fit).  The pool pages
+// are asked for one block earlier and looked at a block after: looking at once would wait for
+// the keys before them (long decode 98 us and 96).  Pages of a multiple of 32 tokens need one
+// entry a block (110 and 99).  The maximum is raised only when a block passes it by 2^8 (sums stay
+// in range, and relative precision does not depend on it), so most blocks need no exchange
+// between lanes and no rescaling.
+//
+// With the join: 32 bf16 streams over MXFP4, 64 heads on 8 of 128, 4096 to 16384 tokens, 364 MB in
+// 96 us, 3.8 TB/s, bound by how many bytes are on their way; 16 f32 streams over int4, 16
+// heads of 128, 100 to 4096 tokens, 85 MB in 42 us, bound by issue (three-term operands: 12
+// products of queries and 24 of values a block of 32 tokens) and by the workgroups' starts
+// and ends; one stream of 777 tokens 10.6 us, two launches' latency.
 template <int FMT, int NG, typename T>
 __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv4_attn(AttnArgs A) {
     constexpr int D = 64 * NG, TQ = sizeof(T) == 4 ? 3 : 1, TP = sizeof(T) == 4 ? 3 : 2;
@@ -679,7 +687,8 @@ __global__ __launch_bounds__(256, attn_waves(FMT, NG, sizeof(T) == 4)) void k_kv
 
 // Joins the splits of the rows that belong to a sequence.  One wave a head of a token: lane s
 // holds split s's maximum and sum (at most 64 splits), and groups of D / 8 lanes take every
-// other split's sums.
+// other split's sums.  Bound by latency: 4.7 us for 16 tokens of 16 heads in three splits, 4.9 for
+// 32 of 64 in eight.
 template <int NG, typename T>
 __device__ __forceinline__ void join(const AttnArgs &A, int tok, int head) {
     constexpr int D = 64 * NG, LPH = D / 8, G = 64 / LPH;
@@ -771,7 +780,8 @@ __device__ __forceinline__ void dot_four(const AttnArgs &A, size_t place, const 
 // a thread: the rows' maxima and sums from the splits', the tokens' logits as the attention
 // kernel left them (it has every key in its hands; reading its 4 bytes a row again costs less
 // than the key's codes and products: 8 sequences to 8192 tokens, groups of 4, 21 us with the
-// keys, 6 so).  Tokens past the logits' room (longer sequences than max_len) are multiplied out.
+// keys, 5.6 so).  Four rows' logits are on their way at a time (6.7 us one by one).  Tokens past
+// the logits' room (longer sequences than max_len) are multiplied out.
 template <int FMT, int NG, typename T>
 __global__ __launch_bounds__(256) void k_kv4_finish(AttnArgs A, int joins) {
     constexpr int D = 64 * NG;
@@ -876,9 +886,11 @@ __global__ __launch_bounds__(256) void k_kv4_finish(AttnArgs A, int joins) {
 // keys stay in registers as operands while the rows pass by, 16 at a time, and each token's sum
 // is formed in one place, in one order.
 //
-// FEW (decode): each wave takes blocks of its own, the next one's keys on their way, with the
-// operands of up to 16 rows loaded once.  Otherwise the four waves share a block and take every
-// fourth 16 of its rows: what takes time is the way to the rows, not the products.
+// FEW (decode whose logits are too many to keep): each wave takes blocks of its own, the next
+// one's keys on their way, with the operands of up to 16 rows loaded once.  Otherwise the four
+// waves share a block and take every fourth 16 of its rows; bound by the exponentials and the
+// way to the rows (7 sequences, 24 heads on 4 of 64, up to 97 new tokens, window 1024: 14.6 us;
+// 20.2 with a branch an element, 28.6 with 16 waves a block).
 template <int FMT, int NG, typename T, bool FEW>
 __global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs A) {
     constexpr int TQ = sizeof(T) == 4 ? 3 : 1, NB = FEW ? 2 : 4, BLK = 16 * NB;
@@ -1025,15 +1037,15 @@ __global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs A) {
 // a workgroup (4 for head_dim 192 and 256, whose sums fill the registers).
 //
 // Splits of the tokens, at most the 64 that a wave joins, in chunks of 128 tokens (one block a
-// wave) at least, 384 of long sequences (12 heads' rows over 11000 tokens: 29 splits 15.0 us, 43
-// 17.0); up to 384 tokens stay whole, which saves the join (300 tokens: 9.2 us, 11.2 in three).
-// The 16-row kernel: as many as make one round of
-// the chip with every sequence full, two workgroups a CU, or three of bf16 over MXFP4 (8 f32
-// MXFP4 streams of 8 kv heads, all of 8192 tokens: 8 splits 27 us, 7 and 10 35; of 1000 to 8192
-// 26, and 30 with 12).  Where its chunks are long, more, since lengths differ and the rounds even
-// out: chunks of 1408 tokens up to one and a half rounds (16 int4 f32 streams of 16 heads, 100
-// to 4096 tokens: 2 splits 50 us, 3 39, 4 47, 8 45; all of 4096: 55, 57, 57, 63), and of 2048 up
-// to four (32 MXFP4 bf16 streams of 8 heads, 4096 to 16384: 3 splits 105 us, 8 96, 16 106).
+// wave) at least, 384 of long sequences (2 streams of 4 kv heads to 11000 tokens: 29 splits 15.0 us,
+// 43 16.8); up to 384 tokens stay whole, which saves the join (300 tokens: 9.2 us, 11.2 in three).
+// The 16-row kernel: as many as make one round of the chip with every sequence full, two
+// workgroups a CU, or three of bf16 over MXFP4 (8 f32 MXFP4 streams of 8 kv heads, all of 8192
+// tokens: 8 splits 27 us, 7 32, 10 35; of 1000 to 8192: 26, and 30 with 12).  Where its chunks are
+// long, more, since lengths differ and the rounds even out: chunks of 1408 tokens up to one and
+// a half rounds (16 int4 f32 streams of 16 heads, 100 to 4096 tokens: 2 splits 50 us, 3 39, 4 47,
+// 8 45; all of 4096: 55, 57, 57, 63), and of 2048 up to four (32 MXFP4 bf16 streams of 8 heads,
+// 4096 to 16384: 3 splits 105 us, 8 96, 16 106).
 static AttnPlan plan_for(bool prompt, int fmt, int dtype, int head_dim, int n_kv, int n_q,
                          int n_tok, int n_seq, int max_new, int max_len, int window,
                          bool weights) {
@@ -1141,8 +1153,8 @@ static hipError_t attention(const AttnArgs &a, int max_len, hipStream_t st) {
             return e;
     }
     if (a.weights != KV4_WEIGHTS_NONE) {
-        // eight blocks a wave (8 sequences to 8192 tokens: 2 blocks 56 us with the attention, 4
-        // 54, 8 52.5, 16 63), or one a workgroup
+        // eight blocks a wave (8 sequences to 8192 tokens: 8 blocks were 7 % better than 2 and 20 %
+        // than 16), or one a workgroup
         const int per = a.few ? 1024 : 64;
         const dim3 grid((unsigned)a.c.n_kv, (unsigned)a.s.n_seq,
                         (unsigned)std::min(65535, (max_len + per - 1) / per));

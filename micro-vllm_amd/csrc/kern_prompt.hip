@@ -21,6 +21,13 @@
 // A tile's scales are prepared by one wave, in turn, two tiles ahead: it takes the powers out,
 // zeroes the scales of tokens that are not there, and gives a token whose value scales are not
 // finite a NaN key (so the rows that see it become NaN, and no others).
+//
+// 2 sequences, 32 heads on 8 of 128, 1024 new tokens over 6000 to 8192, bf16 over int4: 197 GFLOP
+// in 324 us, 607 TFLOP/s, half of what a large matrix product reaches.  What bounds it is that a
+// tile's decoding, products and exponentials cover each other only in part: the vector ALU is
+// busy 51 % of the time and the matrix cores 36 %, two waves a SIMD.  4 waves a workgroup were
+// slower (each decodes twice as much); waves half a tile apart, priorities and interleaved
+// exponentials changed nothing.
 #include "kv4_common.h"
 
 #include <algorithm>
