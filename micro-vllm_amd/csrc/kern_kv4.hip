@@ -547,7 +547,8 @@ __global__ __launch_bounds__(1024) void k_kv4_select(EvictArgs A, int kcap) {
 // One workgroup: 64 slots of one head of one sequence's fresh pages.  The kept rows' codes move
 // in 16-byte pieces, scales and scores after them, each thread's loads all on their way before
 // its first store.  Bound by the rows' scattered reads, 64 bytes each behind three dependent
-// loads (4 sequences, 8 heads of 128 in MXFP4, 8192 rows each kept: 73 MB in 33 us, 2.2 TB/s).
+// loads (4 sequences, 8 heads of 128 in MXFP4, 8192 rows each kept: 73 MB in 33 us, 2.2 TB/s;
+// with 128 or 256 slots a workgroup, more loads on their way, 33 too).
 template <int FMT, int D>
 __global__ __launch_bounds__(256) void k_kv4_move(EvictArgs A) {
     constexpr int CP = D / 32;                          // 16-byte pieces of a row's codes
